@@ -448,31 +448,69 @@ __device__ __forceinline__ void dma16(const __bf16* src, char* lds) {
 }
 
 // MFMA operand fragment of 16 rows (m or n) starting at image row/col `rb`, k-chunk lane >> 4
-template <bool T, int TW = 256>
+// k-contiguous image
 __device__ __forceinline__ bf16x8 frag(const char* img, int rb, int lane) {
-  if constexpr (!T) {
-    const int r = rb + (lane & 15);
-    const int p = (lane >> 4) ^ (((lane >> 3) & 1) << 1);
-    return *reinterpret_cast<const bf16x8*>(img + r * 64 + p * 16);
-  } else {
-    const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
-    const int lc = rb >> 4;
-    const int k0 = 8 * g + q, k1 = k0 + 4;
-    const int h0 = (k0 & 3) | (((k0 >> 3) & 1) << 2), h1 = (k1 & 3) | (((k1 >> 3) & 1) << 2);
-    // inline asm: the intrinsic form makes hipcc wait vmcnt(0) (every DMA in flight) before each transposed read;
-    // the caller waits lgkmcnt(0) itself before the MFMAs (tr_wait)
-    typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-    u32x2 lo, hi;
-    const unsigned a0 = (unsigned)(uintptr_t)(img + k0 * (2 * TW) + ((lc ^ h0) << 5) + 8 * p);
-    const unsigned a1 = (unsigned)(uintptr_t)(img + k1 * (2 * TW) + ((lc ^ h1) << 5) + 8 * p);
-    asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(a0) : "memory");
-    asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(hi) : "v"(a1) : "memory");
-    const u32x2 v8[2] = {lo, hi};
-    bf16x8 out;
-    __builtin_memcpy(&out, v8, 16);
-    return out;
-  }
+  const int r = rb + (lane & 15);
+  const int p = (lane >> 4) ^ (((lane >> 3) & 1) << 1);
+  return *reinterpret_cast<const bf16x8*>(img + r * 64 + p * 16);
 }
+// k-strided image: the LDS address of the fragment's first transposing read; the second is 4 k-rows on, which have the
+// same swizzle (k-row bits 0, 1, 3)
+constexpr int TR_NEXT = 4 * 2 * TM;
+static_assert(TR_NEXT == 2048 && TM == TN, "the offset in TR_READ");
+__device__ __forceinline__ unsigned tr_at(const char* img, int rb, int lane) {
+  const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+  const int k0 = 8 * g + q, h = q | ((g & 1) << 2);
+  return (unsigned)(uintptr_t)(img + k0 * (2 * TM) + (((rb >> 4) ^ h) << 5) + 8 * p);
+}
+// The reads are inline asm: their intrinsic makes hipcc wait vmcnt(0) (every DMA in flight) ahead of each.  The compiler
+// takes an asm statement's outputs as written when it ends and does not count what it reads, so a group's reads and the
+// wait for them are ONE statement, whose outputs are early-clobbered (a read that returns must not overwrite the address of one
+// that has not been issued).
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+struct TrPair {
+  u32x2 lo, hi;
+  __device__ __forceinline__ bf16x8 frag() const { return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3)); }
+};
+#define TR_READ(lo, hi, at) "ds_read_b64_tr_b16 %" #lo ", %" #at "\n\tds_read_b64_tr_b16 %" #hi ", %" #at " offset:2048\n\t"
+#define TR_OUT(t) "=&v"((t).lo), "=&v"((t).hi)
+// 4 fragments of one operand: rows 16 n of the image from column rb
+__device__ __forceinline__ void tr_frags(const char* b, int rb, int lane, bf16x8 (&bfr)[4]) {
+  TrPair t[4];
+  unsigned a[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) a[n] = tr_at(b, rb + 16 * n, lane);
+  asm volatile(TR_READ(0, 1, 8) TR_READ(2, 3, 9) TR_READ(4, 5, 10) TR_READ(6, 7, 11) "s_waitcnt lgkmcnt(0)"
+               : TR_OUT(t[0]), TR_OUT(t[1]), TR_OUT(t[2]), TR_OUT(t[3])
+               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+               : "memory");
+#pragma unroll
+  for (int n = 0; n < 4; ++n) bfr[n] = t[n].frag();
+}
+// 8 fragments of A and 4 of B
+__device__ __forceinline__ void tr_frags(const char* a, int ra, const char* b, int rb, int lane, bf16x8 (&af)[8],
+                                         bf16x8 (&bfr)[4]) {
+  TrPair t[12];
+  unsigned at[12];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) at[i] = tr_at(a, ra + 16 * i, lane);
+#pragma unroll
+  for (int n = 0; n < 4; ++n) at[8 + n] = tr_at(b, rb + 16 * n, lane);
+  asm volatile(TR_READ(0, 1, 24) TR_READ(2, 3, 25) TR_READ(4, 5, 26) TR_READ(6, 7, 27) TR_READ(8, 9, 28) TR_READ(10, 11, 29)
+               TR_READ(12, 13, 30) TR_READ(14, 15, 31) TR_READ(16, 17, 32) TR_READ(18, 19, 33) TR_READ(20, 21, 34)
+               TR_READ(22, 23, 35) "s_waitcnt lgkmcnt(0)"
+               : TR_OUT(t[0]), TR_OUT(t[1]), TR_OUT(t[2]), TR_OUT(t[3]), TR_OUT(t[4]), TR_OUT(t[5]), TR_OUT(t[6]), TR_OUT(t[7]),
+                 TR_OUT(t[8]), TR_OUT(t[9]), TR_OUT(t[10]), TR_OUT(t[11])
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]), "v"(at[8]),
+                 "v"(at[9]), "v"(at[10]), "v"(at[11])
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) af[i] = t[i].frag();
+#pragma unroll
+  for (int n = 0; n < 4; ++n) bfr[n] = t[8 + n].frag();
+}
+#undef TR_READ
+#undef TR_OUT
 
 __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
@@ -503,7 +541,8 @@ __device__ __forceinline__ void wait_tiles(int n) {
 // c * EPI_SP + (r ^ 4 ((c >> 2) & 7)): the b128 writes of 8 lanes (8 columns) and the ds_read2_b32 reads of a row's 4
 // columns (c, c+1, c+2, c+3: dword offsets 0, 68, 136, 204) are both at most 2-way bank-conflicted.
 // The reads are inline asm: hipcc would otherwise wait vmcnt(0) -- the previous iteration's stores -- ahead of every
-// LDS access in a kernel that issues LDS-DMA.  `vec` = every pointer / ldc allows the wide forms.
+// LDS access in a kernel that issues LDS-DMA (each statement waits for its own reads; early-clobbered outputs, as the
+// address serves two).  `vec` = every pointer / ldc allows the wide forms.
 constexpr int EPI_SP = 68;  // staged column pitch (floats)
 __device__ __forceinline__ int epi_sidx(int c, int r) { return c * EPI_SP + (r ^ (((c >> 2) & 7) << 2)); }
 
@@ -513,7 +552,7 @@ __device__ __forceinline__ float4 stage_row4(const float* stage, int c0, int r, 
   f32x2 lo, hi;
   const unsigned a = (unsigned)(uintptr_t)(stage + epi_sidx(c0, r));
   asm volatile("ds_read2_b32 %0, %2 offset1:68\n\tds_read2_b32 %1, %2 offset0:136 offset1:204\n\ts_waitcnt lgkmcnt(0)"
-               : "=v"(lo), "=v"(hi)
+               : "=&v"(lo), "=&v"(hi)
                : "v"(a)
                : "memory");
   return make_float4(lo.x * alpha, lo.y * alpha, hi.x * alpha, hi.y * alpha);
@@ -735,6 +774,7 @@ __device__ __forceinline__ void mainloop(const GemmArgs& g, const int m0, const 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
   const bool row1 = wm == 1;
+  static_assert(!AT || BT, "a k-strided A comes with a k-strided B");
 
   const __bf16* sa[2];
   const __bf16* sb[2];
@@ -773,11 +813,21 @@ __device__ __forceinline__ void mainloop(const GemmArgs& g, const int m0, const 
     // [reads] fragments of tile j
     const char* slot = lds + rd * SLOT_BYTES;
     bf16x8 af[8], bfr[4];
+    if constexpr (AT || BT)  // their reads end with a wait: the DMA is issued first
+      if (j + AHEAD < nk) stage(j + AHEAD, wr);
+    if constexpr (!AT) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) af[i] = frag<AT>(slot, wm * 128 + 16 * i, lane);
+      for (int i = 0; i < 8; ++i) af[i] = frag(slot, wm * 128 + 16 * i, lane);
+    }
+    if constexpr (AT && BT) {
+      tr_frags(slot, wm * 128, slot + OP_BYTES, wn * 64, lane, af, bfr);
+    } else if constexpr (BT) {
+      tr_frags(slot + OP_BYTES, wn * 64, lane, bfr);
+    } else {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) bfr[n] = frag<BT>(slot + OP_BYTES, wn * 64 + 16 * n, lane);
-    if (j + AHEAD < nk) stage(j + AHEAD, wr);
+      for (int n = 0; n < 4; ++n) bfr[n] = frag(slot + OP_BYTES, wn * 64 + 16 * n, lane);
+      if (j + AHEAD < nk) stage(j + AHEAD, wr);
+    }
     GSTAMP(t1);
     if (row1) wait_tiles(min(nk - 1, j + AHEAD) - (j + 1));
     GSTAMP(t2);
@@ -791,10 +841,7 @@ __device__ __forceinline__ void mainloop(const GemmArgs& g, const int m0, const 
 #pragma unroll
         for (int e = 0; e < 8; ++e) rowsum[i] += (float)af[i][e];
     }
-    if constexpr (AT || BT) {  // the transposed reads are inline asm: hipcc does not track them
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    if constexpr (AT || BT) __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < 8; ++i)

@@ -72,7 +72,7 @@ def sources() -> List[Path]:
 # given wrong results now and then on this hardware (the host pass warns that it does not know the feature).  The older
 # kernels keep the code they are tested and tuned with (without packed fp32 the small LSTM step takes 0.184 instead of
 # 0.170 ms).
-NO_PACKED_FP32 = {"mha", "adam_tensors"}
+NO_PACKED_FP32 = {"mha", "adam_tensors", "gemm"}
 
 
 def kernel_flags(src: Path, flags: List[str]) -> List[str]:
