@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <algorithm>
 #include <array>
@@ -1182,9 +1183,12 @@ struct MhaFn : torch::autograd::Function<MhaFn> {
       mha_backward_impl(grads[0], s[0], s[1], s[2], s[3], s[4], s[5].defined() ? OptT(s[5]) : OptT(), ctx->saved_data["causal"].toBool(),
                         ctx->saved_data["scale"].toDouble(), d[0], d[1], d[2]);
     }
-    if (at::GradMode::is_enabled()) {  // create_graph: differentiating these gradients raises
-      auto error = std::make_shared<torch::autograd::DelayedError>("attention: its gradients are not differentiable", 3);
-      d = (*error)(std::move(d));
+    if (at::GradMode::is_enabled()) {
+      // create_graph: differentiating these gradients raises.  The node that does so leads to what they depend on: without
+      // these edges torch.autograd.grad would find no way to q, k, v or dout through it, and leave it out.
+      auto error = std::make_shared<torch::autograd::Error>("attention: its gradients are not differentiable",
+                                                            torch::autograd::collect_next_edges(s[0], s[1], s[2], grads[0]));
+      torch::autograd::set_history(d, error);
     }
     for (int i = 0; i < 3; ++i)
       if (ctx->needs_input_grad(i)) got[i] = d[i];

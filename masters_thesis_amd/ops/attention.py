@@ -126,6 +126,19 @@ def _backward_reference(dout, q, k, v, causal, key_lengths, scale):
     return tuple(g.to(q.dtype) for g in torch.autograd.grad(out, leaves, dout.to(f)))
 
 
+class _Once(torch.autograd.Function):
+    """Gradients as they are; differentiating them raises.  It takes what they depend on too: without a way to it,
+    torch.autograd.grad would leave this node out instead of running it."""
+
+    @staticmethod
+    def forward(ctx, dq, dk, dv, *inputs):
+        return dq.view_as(dq), dk.view_as(dk), dv.view_as(dv)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("attention: its gradients are not differentiable")
+
+
 class _AttentionFn(torch.autograd.Function):
     """The CPU's recorded form (on the GPU: csrc/bindings.cpp MhaFn)."""
 
@@ -138,10 +151,12 @@ class _AttentionFn(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
         q, k, v, out, lse, key_lengths = ctx.saved_tensors
-        grads = attention_backward(dout, q, k, v, out, lse, causal=ctx.causal, key_lengths=key_lengths, scale=ctx.scale)
+        with torch.no_grad():
+            grads = attention_backward(dout, q, k, v, out, lse, causal=ctx.causal, key_lengths=key_lengths, scale=ctx.scale)
+        if torch.is_grad_enabled():  # create_graph
+            grads = _Once.apply(*grads, q, k, v, dout)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
 

@@ -1,0 +1,41 @@
+"""What ops.attention is asked for by autograd beyond first derivatives: raised where it is not there, never left out."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _A():
+    from masters_thesis_amd.ops import attention as A
+
+    return A
+
+
+def leaves(b=2, t=9, h=4, hk=2, d=16, dtype=torch.float32, grad=True):
+    g = torch.Generator(device=DEV).manual_seed(0)
+    return [torch.randn(b, t, n, d, generator=g, device=DEV).to(dtype).requires_grad_(grad) for n in (h, hk, hk)]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_second_derivatives_raise(which):
+    """Also where another differentiable term stands beside the gradients, and in a penalty on them."""
+    x = leaves()
+    out = _A().attention(*x, causal=True)
+    (g,) = torch.autograd.grad(out.square().sum(), x[which], create_graph=True)
+    assert g.requires_grad
+    with pytest.raises(RuntimeError, match="not differentiable"):  # asked for by name: the way to them leads through the gradient
+        torch.autograd.grad(g.square().sum() + out.sum(), x[which], retain_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        (g.square().sum() + out.sum()).backward()
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(_penalty(x), x)
+    # and first derivatives taken with create_graph are those without it
+    (plain,) = torch.autograd.grad(_A().attention(*x, causal=True).square().sum(), x[which])
+    assert torch.equal(g.detach(), plain)
+
+
+def _penalty(x):
+    out = _A().attention(*x)
+    grads = torch.autograd.grad(out.sum(), x, create_graph=True)
+    return out.sum() + sum(g.square().sum() for g in grads)
