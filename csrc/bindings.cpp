@@ -1026,6 +1026,13 @@ void mha_strides(const at::Tensor& t, long (&strides)[3]) {
   for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
 }
 
+// forward-mode derivatives: a tangent would be left behind here
+bool mha_dual(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    if (torch::autograd::isFwGradDefined(*t)) return true;
+  return false;
+}
+
 double mha_check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptT& lens, c10::optional<double> scale) {
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "attention: q, k, v must be (batch, tokens, heads, dim), got ",
                     q.sizes(), ", ", k.sizes(), ", ", v.sizes());
@@ -1048,6 +1055,7 @@ double mha_check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
                           (lens->scalar_type() == at::kInt || lens->scalar_type() == at::kLong),
                       "attention: key_lengths must be int32 or int64 (", q.size(0), ",) on ", q.device(), ", got ", lens->scalar_type(), " ",
                       lens->sizes(), " on ", lens->device());
+  TORCH_CHECK_NOT_IMPLEMENTED(!mha_dual({&q, &k, &v}), "attention: no forward-mode derivatives on the GPU");
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)D);
   TORCH_CHECK_VALUE(s > 0 && std::isfinite(s), "attention: scale must be positive, got ", s);
   return s;
@@ -1175,6 +1183,7 @@ struct MhaFn : torch::autograd::Function<MhaFn> {
     const auto s = ctx->get_saved_variables();
     torch::autograd::variable_list got(6);
     if (!grads[0].defined()) return got;
+    TORCH_CHECK_NOT_IMPLEMENTED(!mha_dual({&grads[0]}), "attention: no forward-mode derivatives on the GPU");
     mha_check_capture();
     torch::autograd::variable_list d(3);
     {
@@ -1221,6 +1230,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mha_backward(const at::Tensor& do
   TORCH_CHECK_VALUE(dout.device() == q.device() && out.device() == q.device() && lse.device() == q.device() &&
                         lse.scalar_type() == at::kFloat,
                     "attention_backward: dout, out and lse (float32) must be on ", q.device());
+  TORCH_CHECK_NOT_IMPLEMENTED(!mha_dual({&dout, &out, &lse}), "attention: no forward-mode derivatives on the GPU");
   at::Tensor d[3];
   const at::Tensor* in[3] = {&q, &k, &v};
   const OptT* given[3] = {&gq, &gk, &gv};

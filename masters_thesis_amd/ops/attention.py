@@ -176,6 +176,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, key_leng
 
     ``return_lse``: also the log-sum-exp (batch, heads, Tq), float32, not differentiable.
 
+    First derivatives only: differentiating the gradients raises, on the GPU also forward-mode derivatives.
+
     Captured into a graph, the backward needs leaves whose earlier graphs are gone: it raises where one is alive on
     another stream.
     """

@@ -39,3 +39,38 @@ def _penalty(x):
     out = _A().attention(*x)
     grads = torch.autograd.grad(out.sum(), x, create_graph=True)
     return out.sum() + sum(g.square().sum() for g in grads)
+
+
+def test_forward_mode_raises():
+    """A tangent is not left behind: every entry point refuses dual tensors, whichever argument carries it."""
+    import torch.autograd.forward_ad as fw
+
+    A = _A()
+    x = leaves(grad=False)
+    out, lse = A.attention_forward(*x)
+    with fw.dual_level():
+        for i in range(3):
+            y = [fw.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(x)]
+            for fn in (A.attention, A.attention_forward):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fn(*y)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            A.attention_backward(fw.make_dual(out, out), *x, out, lse)
+        z = leaves()
+        recorded = A.attention(*z)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(recorded, z, fw.make_dual(out, out))
+
+
+def test_batched_transforms_raise():
+    """torch.func's wrappers, whose tensors have no memory of their own, are refused, not read."""
+    A = _A()
+    x = leaves(grad=False)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(A.attention)(*(t[None] for t in x))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(A.attention, tuple(x), tuple(x))
+    y = leaves()
+    out = A.attention(*y)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, y, torch.stack([out.detach()] * 2), is_grads_batched=True)
