@@ -1280,10 +1280,14 @@ void rope_(at::Tensor x, int64_t seq, int64_t heads, int64_t dim, double base, b
               "rope_: (tokens, columns) on the GPU with heads * dim columns in front");
   TORCH_CHECK(seq > 0 && heads > 0 && dim > 0 && dim % 2 == 0 && dim <= 4096 && base > 0, "rope_: bad sizes");
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat, "rope_: bfloat16 or float32");
+  // the turn is recorded nowhere: gradients through it would miss it
+  TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()) && !mha_dual({&x}),
+              "rope_: in place and without a derivative, so not on a tensor that a gradient passes through");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   const int rc = mta_rope(mha_type(x), x.data_ptr(), x.size(0), (int)seq, x.stride(0), (int)heads, (int)dim, base,
                           inverse ? 1 : 0, cur_stream());
   TORCH_CHECK(rc == 0, "rope_: unsupported size");
+  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();  // a backward that saved x before sees the change
 }
 
 // ------------------------------------------------------------------------------- Adam over a list of tensors

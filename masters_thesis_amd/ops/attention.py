@@ -192,7 +192,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, key_leng
 
 def rope_(x: Tensor, seq: int, heads: int, dim: int, base: float = 10000.0, inverse: bool = False) -> Tensor:
     """Turns the first ``heads * dim`` columns of ``x`` (tokens of ``seq``-long sequences, columns) in place: the pair
-    (2 i, 2 i + 1) of each head by ``position * base^(-2 i / dim)`` (back with ``inverse``).  bfloat16 or float32."""
+    (2 i, 2 i + 1) of each head by ``position * base^(-2 i / dim)`` (back with ``inverse``).  bfloat16 or float32.
+    Not differentiable: a tensor that a gradient passes through is refused (its gradient is turned with ``inverse`` by
+    whoever keeps the graph, as the encoder does)."""
     if not use_hip(x):
         raise ValueError("rope_ is the GPU form: on the CPU use ops.extras.rope_reference")
     lib().rope_(x, int(seq), int(heads), int(dim), float(base), bool(inverse))

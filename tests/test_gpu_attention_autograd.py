@@ -74,3 +74,31 @@ def test_batched_transforms_raise():
     out = A.attention(*y)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(out, y, torch.stack([out.detach()] * 2), is_grads_batched=True)
+
+
+def test_rope_is_refused_within_a_graph():
+    """It records nothing: the gradients of what it turned would be those of what it did not."""
+    import torch.autograd.forward_ad as fw
+
+    A = _A()
+    w = torch.randn(6, 24, device=DEV, requires_grad=True)
+    x = torch.randn(10, 6, device=DEV)
+    for t in (w, x @ w, (x @ w)[:, :16]):
+        with pytest.raises(RuntimeError, match="gradient"):
+            A.rope_(t, 5, 2, 4)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="gradient"):
+        A.rope_(fw.make_dual(w.detach(), w.detach()), 5, 2, 4)
+    with torch.no_grad():  # as any operation in place
+        A.rope_(w, 3, 2, 4)
+    with torch.inference_mode():
+        A.rope_(torch.randn(6, 24, device=DEV), 3, 2, 4)
+
+
+def test_rope_is_seen_by_a_backward_that_saved_its_tensor():
+    A = _A()
+    x = torch.randn(10, 24, device=DEV)
+    w = torch.randn(24, device=DEV, requires_grad=True)
+    y = (x * w).sum()
+    A.rope_(x, 5, 2, 4)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
