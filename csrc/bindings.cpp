@@ -1278,7 +1278,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mha_backward(const at::Tensor& do
 void rope_(at::Tensor x, int64_t seq, int64_t heads, int64_t dim, double base, bool inverse) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= heads * dim && x.size(1) >= heads * dim,
               "rope_: (tokens, columns) on the GPU with heads * dim columns in front");
-  TORCH_CHECK(seq > 0 && heads > 0 && dim > 0 && dim % 2 == 0 && dim <= 4096 && base > 0, "rope_: bad sizes");
+  TORCH_CHECK(seq > 0 && seq <= 0x7fffffff && heads > 0 && dim > 0 && dim % 2 == 0 && dim <= 4096 && base > 0, "rope_: bad sizes");
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat, "rope_: bfloat16 or float32");
   // the turn is recorded nowhere: gradients through it would miss it
   TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()) && !mha_dual({&x}),

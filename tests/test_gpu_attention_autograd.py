@@ -94,6 +94,19 @@ def test_rope_is_refused_within_a_graph():
         A.rope_(torch.randn(6, 24, device=DEV), 3, 2, 4)
 
 
+def test_rope_of_sequences_past_31_bits():
+    """Lengths are 32-bit numbers in the kernel: longer ones are refused, not cut (2^32 would become 0)."""
+    A = _A()
+    x = torch.randn(6, 24, device=DEV)
+    for seq in (2 ** 32, 2 ** 32 + 3, 2 ** 31, 0, -1):
+        with pytest.raises(RuntimeError, match="bad sizes"):
+            A.rope_(x, seq, 2, 4)
+    y = x.clone()
+    A.rope_(x, 2 ** 31 - 1, 2, 4)
+    A.rope_(y, 6, 2, 4)
+    assert torch.equal(x, y)
+
+
 def test_rope_is_seen_by_a_backward_that_saved_its_tensor():
     A = _A()
     x = torch.randn(10, 24, device=DEV)
