@@ -1095,7 +1095,8 @@ void mha_launch(MhaArgs& A, const at::Tensor& q, bool backward) {
     A.part = part.data_ptr<float>();
   }
   const int rc = mta_mha(type, backward ? 1 : 0, &A, cur_stream());
-  TORCH_CHECK(rc == 0, "attention: unsupported size (rc=", rc, ")");
+  TORCH_CHECK(rc != 2, "attention: too large for one launch: q ", q.sizes(), ", ", A.Tk, " keys in ", A.Hkv, " heads");
+  TORCH_CHECK(rc == 0, "attention: not launched (rc=", rc, ")");
 }
 
 // (out, lse or undefined)
@@ -1286,7 +1287,7 @@ void rope_(at::Tensor x, int64_t seq, int64_t heads, int64_t dim, double base, b
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   const int rc = mta_rope(mha_type(x), x.data_ptr(), x.size(0), (int)seq, x.stride(0), (int)heads, (int)dim, base,
                           inverse ? 1 : 0, cur_stream());
-  TORCH_CHECK(rc == 0, "rope_: unsupported size");
+  TORCH_CHECK(rc == 0, "rope_: not launched (rc=", rc, ")");
   if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();  // a backward that saved x before sees the change
 }
 

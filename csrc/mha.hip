@@ -1400,15 +1400,16 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(T* x, long tokens, int se
   }
 }
 
-template <typename K>
-int launch(K kernel, long grid, int lds, const MhaArgs& A, hipStream_t st) {
-  if (grid < 1 || grid > 0x7fffffffL) return 2;
-  if (lds > 64 * 1024 &&
-      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-    return 3;
-  kernel<<<(unsigned)grid, THREADS, lds, st>>>(A);
-  return 0;
+// 0, or why a kernel was not started: 2 more threads than a launch holds (2^32 - 1), 3 the LDS, 4 the launch itself
+template <typename... P>
+int start(void (*kernel)(P...), long grid, int lds, hipStream_t st, P... args) {
+  if (grid < 1 || grid > 0xffffffffL / THREADS) return 2;
+  const void* f = reinterpret_cast<const void*>(kernel);
+  if (lds > 64 * 1024 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return 3;
+  void* p[] = {&args...};
+  return hipLaunchKernel(f, dim3((unsigned)grid), dim3(THREADS), p, lds, st) == hipSuccess ? 0 : 4;
 }
+int launch(void (*kernel)(MhaArgs), long grid, int lds, const MhaArgs& A, hipStream_t st) { return start<MhaArgs>(kernel, grid, lds, st, A); }
 
 // keys of a tile of the many-row kernels, rows of one of the many-key kernel
 template <typename T>
@@ -1466,8 +1467,7 @@ int fwd(const MhaArgs& A, hipStream_t st) {
   const long R = (long)A.G * A.Tq, P = (long)A.B * A.Hkv;
   if (!few(P, R)) return launch(mha_fwd_kernel<T, DP, BN>, grid_of(P, (R + 127) / 128), 4 * BN * ROW, A, st);
   const int rc = launch(mha_few_kernel<T, DP>, grid_of(P, (R + 31) / 32 * A.splits), OWN > 20 * 1024 ? OWN : 20 * 1024, A, st);
-  if (rc == 0 && A.splits > 1) mha_join_kernel<T><<<(unsigned)((R * P + WAVES - 1) / WAVES), THREADS, 0, st>>>(A);
-  return rc;
+  return rc == 0 && A.splits > 1 ? launch(mha_join_kernel<T>, (R * P + WAVES - 1) / WAVES, 0, A, st) : rc;
 }
 
 template <typename T, int DP>
@@ -1506,12 +1506,7 @@ int bwd(const MhaArgs& A, hipStream_t st) {
     add(part, A.dk, A.dks, A.kv_splits, 2 * all, A.Tk, 1, A.scale);
     add(part + all, A.dv, A.dvs, A.kv_splits, 2 * all, A.Tk, 1, 1.f);
   }
-  if (S.n) {
-    const long grid = (items + THREADS - 1) / THREADS;
-    if (grid > 0x7fffffffL) return 2;
-    mha_sum_kernel<T><<<(unsigned)grid, THREADS, 0, st>>>(S);
-  }
-  return 0;
+  return S.n ? start<Sums>(mha_sum_kernel<T>, (items + THREADS - 1) / THREADS, 0, st, S) : 0;
 }
 
 template <typename T>
@@ -1560,10 +1555,8 @@ extern "C" int mta_rope(int dtype, void* x, long tokens, int seq, long ld, int h
   const long n = tokens * (D / 2);
   if (n <= 0) return 0;
   const long grid = (n + THREADS - 1) / THREADS;
-  if (grid > 0x7fffffffL) return 2;
   const float s = inverse ? -1.f : 1.f;
-  if (dtype == MHA_BF16) rope_kernel<__bf16><<<(unsigned)grid, THREADS, 0, st>>>((__bf16*)x, tokens, seq, ld, heads, D, base, s);
-  else if (dtype == MHA_F32) rope_kernel<float><<<(unsigned)grid, THREADS, 0, st>>>((float*)x, tokens, seq, ld, heads, D, base, s);
-  else return 1;
-  return 0;
+  if (dtype == MHA_BF16) return start(rope_kernel<__bf16>, grid, 0, st, (__bf16*)x, tokens, seq, ld, heads, D, base, s);
+  if (dtype == MHA_F32) return start(rope_kernel<float>, grid, 0, st, (float*)x, tokens, seq, ld, heads, D, base, s);
+  return 1;
 }
