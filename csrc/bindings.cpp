@@ -163,6 +163,7 @@ void mta_prefetch_destroy(void* h);
 // mha.hip (attention for sequences of any length), adam_tensors.hip (Adam over a list of tensors)
 long mta_mha_plan(int dtype, int backward, MhaArgs* A);
 int mta_mha(int dtype, int backward, MhaArgs* A, hipStream_t st);
+int mta_mha_meet(const MhaBox* a, const MhaBox* b);
 int mta_rope(int dtype, void* x, long tokens, int seq, long ld, int heads, int D, double base, int inverse,
              hipStream_t st);
 int mta_adam_group(long elements);
@@ -1233,6 +1234,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mha_backward(const at::Tensor& do
                     "attention_backward: dout, out and lse (float32) must be on ", q.device());
   TORCH_CHECK_NOT_IMPLEMENTED(!mha_dual({&dout, &out, &lse}), "attention: no forward-mode derivatives on the GPU");
   at::Tensor d[3];
+  const auto box = [](const at::Tensor& t) {
+    MhaBox x{(long)(reinterpret_cast<uintptr_t>(t.data_ptr()) / t.element_size()), {}, {}};
+    for (int j = 0; j < 4; ++j) x.strides[j] = t.stride(j), x.sizes[j] = t.size(j);
+    return x;
+  };
   const at::Tensor* in[3] = {&q, &k, &v};
   const OptT* given[3] = {&gq, &gk, &gv};
   for (int i = 0; i < 3; ++i) {
@@ -1267,9 +1273,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mha_backward(const at::Tensor& do
       TORCH_CHECK_VALUE(own.second <= other.first || other.second <= own.first, "attention_backward: gradient ", i,
                         " lies in the memory of an input");
     }
-    for (int j = 0; j < i; ++j)
-      TORCH_CHECK_VALUE(d[j].numel() == 0 || d[i].data_ptr() != d[j].data_ptr(), "attention_backward: gradients ", j, " and ", i,
-                        " share memory");
+    for (int j = 0; j < i; ++j) {  // views of one buffer may lie between each other
+      const MhaBox a = box(d[j]), b = box(d[i]);
+      TORCH_CHECK_VALUE(!has(*given[j]) || !mta_mha_meet(&a, &b), "attention_backward: gradients ", j, " and ", i, " share memory");
+    }
   }
   mha_backward_impl(dout, q, k, v, out, lse, lens, causal, s, d[0], d[1], d[2]);
   return {d[0], d[1], d[2]};

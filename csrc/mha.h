@@ -28,3 +28,8 @@ struct MhaArgs {
   int dq_splits, dq_split_tiles;  // the same of the dQ kernel
   int kv_splits;    // row ranges a key tile is split over (dK, dV kernel)
 };
+
+// elements of a tensor with 4 dimensions: `at` of the first, strides and sizes, in elements
+struct MhaBox {
+  long at, strides[4], sizes[4];
+};

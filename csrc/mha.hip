@@ -1550,6 +1550,51 @@ extern "C" int mta_mha(int dtype, int backward, MhaArgs* A, hipStream_t st) {
   return 1;
 }
 
+// Whether two tensors (strides >= 0) have an element in common: whole numbers x, each in its range, with
+// sum stride * x = b.at - a.at, where a dimension of `a` counts up and one of `b` down, and equal strides are one x.  By
+// descending stride, x is taken only where the smaller strides can make up the rest, which for dimensions that lie within
+// each other are two values or three.  1 also where the search does not end within its steps.
+extern "C" int mta_mha_meet(const MhaBox* a, const MhaBox* b) {
+  struct Axis {
+    long stride, lo, hi;
+  } axes[8];
+  int n = 0;
+  auto add = [&](long stride, long lo, long hi) {
+    if (lo == hi) return;
+    int i = 0;
+    while (i < n && axes[i].stride > stride) ++i;
+    if (i == n || axes[i].stride != stride) {
+      for (int j = n++; j > i; --j) axes[j] = axes[j - 1];
+      axes[i] = Axis{stride, 0, 0};
+    }
+    axes[i].lo += lo;
+    axes[i].hi += hi;
+  };
+  for (int k = 0; k < 4; ++k) {
+    if (a->sizes[k] == 0 || b->sizes[k] == 0) return 0;
+    if (a->strides[k]) add(a->strides[k], 0, a->sizes[k] - 1);
+    if (b->strides[k]) add(b->strides[k], 1 - b->sizes[k], 0);
+  }
+  long least[9] = {}, most[9] = {};  // of axes i ..
+  for (int i = n - 1; i >= 0; --i) {
+    least[i] = least[i + 1] + axes[i].stride * axes[i].lo;
+    most[i] = most[i + 1] + axes[i].stride * axes[i].hi;
+  }
+  int steps = 1 << 16;
+  auto down = [](long x, long y) { return x / y - (x % y != 0 && x < 0); };  // y > 0
+  auto search = [&](auto&& self, int i, long rest) -> bool {
+    if (i == n) return rest == 0;
+    const Axis& x = axes[i];
+    long from = -down(most[i + 1] - rest, x.stride), to = down(rest - least[i + 1], x.stride);
+    from = from > x.lo ? from : x.lo;
+    to = to < x.hi ? to : x.hi;
+    for (long v = from; v <= to; ++v)
+      if (--steps < 0 || self(self, i + 1, rest - x.stride * v)) return true;
+    return false;
+  };
+  return search(search, 0, b->at - a->at);
+}
+
 extern "C" int mta_rope(int dtype, void* x, long tokens, int seq, long ld, int heads, int D, double base, int inverse,
                         hipStream_t st) {
   const long n = tokens * (D / 2);

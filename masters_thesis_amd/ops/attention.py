@@ -98,17 +98,45 @@ def attention_forward(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, 
         return out.to(q.dtype).contiguous(), (lse if need_lse else None)
 
 
+def _check_grads(grads, ins, others) -> None:
+    """Places to write gradients into, on the CPU (on the GPU: csrc/bindings.cpp mha_backward)."""
+    places = []
+    for i, (g, x) in enumerate(zip(grads, ins)):
+        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
+            raise ValueError(f"attention_backward: gradient {i} must be {tuple(x.shape)} {x.dtype} on {x.device}")
+        if not g.numel():
+            continue
+        unit = 16 // g.element_size()
+        if g.stride(3) != 1 or g.data_ptr() % 16 or any(n > 1 and (s <= 0 or s % unit) for s, n in zip(g.stride()[:3], g.shape)):
+            raise ValueError(f"attention_backward: gradient {i} must have contiguous rows that start on 16 bytes")
+        at = torch.full((1,), g.data_ptr() // g.element_size())
+        for s, n in zip(g.stride(), g.shape):
+            at = (at[:, None] + s * torch.arange(n)).view(-1)
+        lo, hi = int(at.min()) * g.element_size(), (int(at.max()) + 1) * g.element_size()
+        for t in others:
+            if t.numel():
+                end = t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+                if lo < end and t.data_ptr() < hi:
+                    raise ValueError(f"attention_backward: gradient {i} lies in the memory of an input")
+        places.append(at)
+    if places and torch.cat(places).unique().numel() < sum(at.numel() for at in places):
+        raise ValueError("attention_backward: elements of the gradients share memory")
+
+
 def attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, *, causal: bool = False,
                        key_lengths: Optional[Tensor] = None, scale: Optional[float] = None,
                        grads: Optional[Tuple[Tensor, Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """Gradients ``(dq, dk, dv)`` of :func:`attention` from its output and log-sum-exp.  ``grads``: tensors to write
-    them into (any strides with 16-byte rows, for instance views of one packed buffer; not the inputs' memory)."""
+    them into (any strides with 16-byte rows, for instance views of one packed buffer; neither each other's memory nor the
+    inputs')."""
     if use_hip(q):
         return lib().mha_backward(dout, q, k, v, out, lse, key_lengths, causal, scale, *(grads or (None, None, None)))
     scale = _check(q, k, v, key_lengths, scale)
     if dout.shape != q.shape or out.shape != q.shape or lse.shape != (q.shape[0], q.shape[2], q.shape[1]):
         raise ValueError(f"attention_backward: dout {tuple(dout.shape)} and out {tuple(out.shape)} must be {tuple(q.shape)}, "
                          f"lse {tuple(lse.shape)} (batch, heads, queries)")
+    if grads is not None:
+        _check_grads(grads, (q, k, v), (dout, q, k, v, out, lse))
     got = _backward_reference(dout, q, k, v, causal, key_lengths, scale)
     if grads is None:
         return got

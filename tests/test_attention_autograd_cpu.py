@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from masters_thesis_amd.ops.attention import attention
+from masters_thesis_amd.ops.attention import attention, attention_backward, attention_forward
 
 
 def leaves(b=2, t=9, h=4, hk=2, d=16):
@@ -23,3 +23,26 @@ def test_second_derivatives_raise(which):
         (g.square().sum() + out.sum()).backward()
     (plain,) = torch.autograd.grad(attention(*x, causal=True).square().sum(), x[which])
     assert torch.equal(g.detach(), plain)
+
+
+def test_gradients_into_shared_memory_are_refused():
+    q, k, v = (x.detach() for x in leaves(2, 8, 2, 2, 32))
+    do = torch.randn_like(q)
+    out, lse = attention_forward(q, k, v)
+    new = lambda: [torch.zeros_like(x) for x in (q, k, v)]  # noqa: E731
+    packed = torch.zeros(2, 8, 6, 32)
+    for bad in ((packed[:, :, :2], packed[:, :, 1:3], packed[:, :, 4:]), (packed[:, :, :2], packed[:, :, 2:4], packed[:, :, 3:5])):
+        with pytest.raises(ValueError, match="memory"):
+            attention_backward(do, q, k, v, out, lse, grads=bad)
+    for i, bad in ((0, q), (1, do), (2, out), (1, torch.zeros_like(k).as_strided(k.shape, (16 * 32, 32, 32, 1)))):
+        grads = new()
+        grads[i] = bad
+        with pytest.raises(ValueError, match="memory"):
+            attention_backward(do, q, k, v, out, lse, grads=tuple(grads))
+    for i, bad in ((0, q[:1].clone()), (1, k.double()), (2, torch.zeros(2, 8, 2, 33)[..., :32])):
+        grads = new()
+        grads[i] = bad
+        with pytest.raises(ValueError):
+            attention_backward(do, q, k, v, out, lse, grads=tuple(grads))
+    attention_backward(do, q, k, v, out, lse, grads=(packed[:, :, :2], packed[:, :, 2:4], packed[:, :, 4:]))
+    assert all(torch.equal(a, b) for a, b in zip(packed.split(2, 2), attention_backward(do, q, k, v, out, lse)))

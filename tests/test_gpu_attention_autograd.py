@@ -115,3 +115,20 @@ def test_rope_is_seen_by_a_backward_that_saved_its_tensor():
     A.rope_(x, 5, 2, 4)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_gradients_that_overlap_are_refused():
+    """Views of one buffer a head apart (two kernels would write the same places) are refused, beside each other they are not."""
+    A = _A()
+    q, k, v = leaves(2, 8, 2, 2, 32, grad=False)
+    do = torch.randn_like(q)
+    out, lse = A.attention_forward(q, k, v)
+    packed = torch.zeros(2, 8, 6, 32, device=DEV)
+    for bad in ((packed[:, :, :2], packed[:, :, 1:3], packed[:, :, 4:]), (packed[:, :, :2], packed[:, :, 2:4], packed[:, :, 3:5]),
+                (packed[:, :, 3:5], packed[:, :, :2], packed[:, :, 4:])):
+        with pytest.raises(ValueError, match="memory"):
+            A.attention_backward(do, q, k, v, out, lse, grads=bad)
+    turned = torch.zeros(6, 2, 8, 32, device=DEV).permute(1, 2, 0, 3)  # heads first
+    for p in (packed, turned):
+        A.attention_backward(do, q, k, v, out, lse, grads=(p[:, :, :2], p[:, :, 2:4], p[:, :, 4:]))
+        assert all(torch.equal(a, b) for a, b in zip(p.split(2, 2), A.attention_backward(do, q, k, v, out, lse)))
