@@ -1006,6 +1006,11 @@ void attention_f32(bool bwd, at::Tensor qkv, at::Tensor out, at::Tensor lse, con
               ")");
 }
 
+// after a write through a tensor's pointer: a backward that saved it before sees the change
+void bump_version(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ------------------------------------------------------------------------------- attention of any length (csrc/mha.hip)
 int mha_type(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -1279,6 +1284,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mha_backward(const at::Tensor& do
     }
   }
   mha_backward_impl(dout, q, k, v, out, lse, lens, causal, s, d[0], d[1], d[2]);
+  for (int i = 0; i < 3; ++i)
+    if (has(*given[i])) bump_version(d[i]);
   return {d[0], d[1], d[2]};
 }
 
@@ -1295,7 +1302,7 @@ void rope_(at::Tensor x, int64_t seq, int64_t heads, int64_t dim, double base, b
   const int rc = mta_rope(mha_type(x), x.data_ptr(), x.size(0), (int)seq, x.stride(0), (int)heads, (int)dim, base,
                           inverse ? 1 : 0, cur_stream());
   TORCH_CHECK(rc == 0, "rope_: not launched (rc=", rc, ")");
-  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();  // a backward that saved x before sees the change
+  bump_version(x);
 }
 
 // ------------------------------------------------------------------------------- Adam over a list of tensors

@@ -132,3 +132,16 @@ def test_gradients_that_overlap_are_refused():
     for p in (packed, turned):
         A.attention_backward(do, q, k, v, out, lse, grads=(p[:, :, :2], p[:, :, 2:4], p[:, :, 4:]))
         assert all(torch.equal(a, b) for a, b in zip(p.split(2, 2), A.attention_backward(do, q, k, v, out, lse)))
+
+
+def test_gradients_written_in_place_are_seen_by_a_backward_that_saved_them():
+    A = _A()
+    q, k, v = leaves(2, 8, 2, 2, 32, grad=False)
+    out, lse = A.attention_forward(q, k, v)
+    grads = tuple(torch.zeros_like(x) for x in (q, k, v))
+    w = torch.ones(3, device=DEV, requires_grad=True)
+    y = [(g * w[i]).sum() for i, g in enumerate(grads)]
+    A.attention_backward(out, q, k, v, out, lse, grads=grads)
+    for x in y:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            x.backward()
