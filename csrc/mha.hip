@@ -1103,6 +1103,7 @@ struct RowTiles {
   typedef Stage<T, DP, BR, NT> ST;
   const MhaArgs& A;
   const int b, hk, n, R, e0, per_pass, me;
+  const int blind;  // rows in front that see no key: they are staged as zeros, whatever they hold
   const bool even;  // G divides the rows of a pass: a thread's rows are the same query head's, and their tokens a step apart
   const T *qp, *dop;
   ST sq, sdo;
@@ -1111,7 +1112,7 @@ struct RowTiles {
 
   __device__ __forceinline__ RowTiles(const MhaArgs& A, int b, int hk, int n)
       : A(A), b(b), hk(hk), n(n), R(A.G * A.Tq), e0(ST::elem(A.D)), per_pass(ST::RPI / A.G), me(threadIdx.x % NT),
-        even(ST::RPI % A.G == 0) {
+        blind(A.causal && A.Tq > A.Tk ? A.G * (A.Tq - A.Tk) : 0), even(ST::RPI % A.G == 0) {
     const int t0 = token_of(A, ST::row()), h0 = hk * A.G + ST::row() - t0 * A.G;
     qp = at<T>(A.q, A.qs, b, t0, h0) + e0;
     dop = at<T>(A.dout, A.dos, b, t0, h0) + e0;
@@ -1146,7 +1147,12 @@ struct RowTiles {
     }
   }
   // Q rows, dO rows, then L log2(e), delta, the keys each row sees; max |dO| (SCALED)
-  __device__ __forceinline__ void put(unsigned t) const {
+  __device__ __forceinline__ void put(unsigned t, int it) {
+    if (it * BR < blind) {
+#pragma unroll
+      for (int i = 0; i < ST::N; ++i)
+        if (it * BR + ST::row() + i * ST::RPI < blind) sq.r[i] = sdo.r[i] = u32x4{};
+    }
     sq.store(t);
     sdo.store(t + TILE);
     if (me < BR) {
@@ -1158,7 +1164,7 @@ struct RowTiles {
     if constexpr (SCALED<T>) {
       static_assert(BR <= 64, "the rows' maximum is one wave's");
       if (me < 64) {
-        float top = st_top;
+        float top = st_see > 0 ? st_top : 0.f;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
         if (me == 0) lds_put(t + 2 * TILE + 12 * BR, top);
@@ -1259,7 +1265,7 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dkv_kernel
     RowTiles<T, DP, BR, THREADS> rows(A, b, hk, n);
     if (it0 < it1) {
       rows.fetch(it0);
-      rows.put(lds);
+      rows.put(lds, it0);
     }
     mta_wait_vmem();  // the keys' operands too: a wait for them inside the loop would wait for the next tile as well
     __syncthreads();
@@ -1268,7 +1274,7 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dkv_kernel
       for (int it = from; it < to; ++it) {
         if (it + 1 < it1) rows.fetch(it + 1);
         w.template tile<BR, decltype(masked)::value>(lds + ((it - it0) & 1) * BUF, c, key, A.D, lane);
-        if (it + 1 < it1) rows.put(lds + ((it + 1 - it0) & 1) * BUF);
+        if (it + 1 < it1) rows.put(lds + ((it + 1 - it0) & 1) * BUF, it + 1);
         __syncthreads();
       }
     };
@@ -1321,7 +1327,7 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dkv_few_ke
   const unsigned qt = lds + wave * BUF;
   if (it < x.it1) rows.fetch(it);
   for (; it < x.it1; it += WAVES) {
-    rows.put(qt);
+    rows.put(qt, it);
     wave_order();
     if (it + WAVES < x.it1) rows.fetch(it + WAVES);
     if (it < x.all) w.template tile<32, true>(qt, A.scale * LOG2E, key, A.D, lane);
