@@ -148,6 +148,8 @@ def attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tenso
 
 def _backward_reference(dout, q, k, v, causal, key_lengths, scale):
     f = torch.float32
+    sees = _seen(q, k, causal, key_lengths).any(-1)[:, 0, :, None, None]  # (batch or 1, Tq, 1, 1)
+    q, dout = (torch.where(sees, t, torch.zeros((), dtype=t.dtype, device=t.device)) for t in (q, dout))  # others take no part
     leaves = [t.detach().to(f).requires_grad_() for t in (q, k, v)]
     with torch.enable_grad():
         out, _ = attention_reference(*leaves, causal=causal, key_lengths=key_lengths, scale=scale)

@@ -1,4 +1,6 @@
 """What ops.attention is asked for by autograd beyond first derivatives, on the CPU."""
+import math
+
 import pytest
 import torch
 
@@ -46,3 +48,20 @@ def test_gradients_into_shared_memory_are_refused():
             attention_backward(do, q, k, v, out, lse, grads=tuple(grads))
     attention_backward(do, q, k, v, out, lse, grads=(packed[:, :, :2], packed[:, :, 2:4], packed[:, :, 4:]))
     assert all(torch.equal(a, b) for a, b in zip(packed.split(2, 2), attention_backward(do, q, k, v, out, lse)))
+
+
+def test_what_blind_rows_hold_reaches_nothing():
+    """Causal, more queries than keys: the first ones see no key, and their q and dout may be anything."""
+    g = torch.Generator().manual_seed(1)
+    q, do = (torch.randn(2, 9, 4, 16, generator=g) for _ in range(2))
+    k, v = (torch.randn(2, 4, 2, 16, generator=g) for _ in range(2))
+    q[:, :5], do[:, :5] = 0, 0
+
+    def run():
+        out, lse = attention_forward(q, k, v, causal=True)
+        return out, *attention_backward(do, q, k, v, out, lse, causal=True)
+
+    want = run()
+    for bad in (math.nan, math.inf):
+        q[:, :5:2], do[:, 1:5], do[:, 0] = bad, bad, bad
+        assert all(torch.equal(a, b) for a, b in zip(run(), want))
