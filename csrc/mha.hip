@@ -664,7 +664,7 @@ constexpr int backward_waves(int dp) {
 
 // float16 holds P and dS = P (dP - delta) poorly where P or dO is small (below 2^-14 in steps of 2^-24), and dS not at
 // all past 65504.  There P is kept times 2^12 for dV (by a shift of its exponent), and dS times a power of two that takes
-// max |dO|, of the row (dQ) or of the rows so far (dK), to 2 .. 4; the sums are divided by them.  Weights stay normal down
+// max |dO|, of the row (dQ) or of the rows so far that see the key (dK), to 2 .. 4; the sums are divided by them.  Weights stay normal down
 // to 2^-26 and 2^-15; dS overflows only past |dP| of 16000 max |dO|, where V's rows add up to as much.
 template <typename T>
 constexpr bool SCALED = sizeof(T) == 2 && !std::is_same_v<T, __bf16>;
@@ -988,7 +988,7 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dq_few_ker
 
 template <typename T, int DP, int BR>
 constexpr int dkv_buffer() {
-  return (2 * BR * DP * (int)sizeof(T) + 3 * BR * 4 + 4 + 1023) / 1024 * 1024;
+  return (2 * BR * DP * (int)sizeof(T) + (SCALED<T> ? 4 * BR + 1 : 3 * BR) * 4 + 1023) / 1024 * 1024;
 }
 
 // ---- backward, dK and dV: one tile of BR rows against a wave's 32 keys --------------------------------------------------
@@ -1146,7 +1146,7 @@ struct RowTiles {
       st_see = 0;
     }
   }
-  // Q rows, dO rows, then L log2(e), delta, the keys each row sees; max |dO| (SCALED)
+  // Q rows, dO rows, then L log2(e), delta, the keys each row sees; (SCALED) each row's max |dO|, the tile's
   __device__ __forceinline__ void put(unsigned t, int it) {
     if (it * BR < blind) {
 #pragma unroll
@@ -1165,9 +1165,10 @@ struct RowTiles {
       static_assert(BR <= 64, "the rows' maximum is one wave's");
       if (me < 64) {
         float top = st_see > 0 ? st_top : 0.f;
+        if (me < BR) lds_put(t + 2 * TILE + 12 * BR + 4 * me, top);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        if (me == 0) lds_put(t + 2 * TILE + 12 * BR, top);
+        if (me == 0) lds_put(t + 2 * TILE + 16 * BR, top);
       }
     }
   }
@@ -1178,7 +1179,8 @@ template <typename T, int DP>
 struct GradKeys {
   typename El<T>::frag k[DP / 16], v[DP / 16];
   f32x16 dk[DP / 32], dv[DP / 32];
-  float times = exp2f(-SHIFT), top = 0.f;  // SCALED: dS is 2^12 P times (dP - delta) times this; the rows' maximum so far
+  // SCALED, of the lane's key: dS is 2^12 P times (dP - delta) times this; the maximum so far of the rows that see the key
+  float times = exp2f(-SHIFT), top = 0.f;
 
   __device__ __forceinline__ void start(const MhaArgs& A, int b, int hk, int key, bool real, int h) {
     load_frags<T, DP>(k, real ? at<T>(A.k, A.ks, b, key, hk) : nullptr, A.D, h);
@@ -1190,17 +1192,29 @@ struct GradKeys {
   __device__ __forceinline__ void tile(unsigned qt, float c, int key, int D, int lane) {
     constexpr int TILE = BR * Tile<T, DP>::ROW_BYTES;
     if constexpr (SCALED<T>) {
-      const float now = mta_readlane(lds_get<float>(qt + 2 * TILE + 12 * BR), 0);
-      if (now > top) {
-        const float next = ds_scale(now) * exp2f(-SHIFT), by = next / times;
-        if (by != 1.f) {
+      const unsigned f = qt + 2 * TILE;
+      float now = 0.f;
+      if constexpr (MASKED) {
+#pragma unroll 4
+        for (int r = 0; r < BR; r += 4) {
+          const f32x4 x = lds_get<f32x4>(f + 12 * BR + 4 * r);
+          const u32x4 sees = lds_get<u32x4>(f + 8 * BR + 4 * r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) now = fmaxf(now, key < (int)sees[j] ? x[j] : 0.f);
+        }
+      } else {
+        now = lds_get<float>(f + 16 * BR);
+      }
+      if (__any(now > top)) {
+        const float next = now > top ? ds_scale(now) * exp2f(-SHIFT) : times, by = next / times;
+        if (__any(by != 1.f)) {
 #pragma unroll
           for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dk[d][r] *= by;
         }
         times = next;
-        top = now;
+        top = fmaxf(top, now);
       }
     }
     dkv_tile<T, DP, BR, MASKED>(qt, qt + TILE, qt + 2 * TILE, k, v, dk, dv, c, times, key, D, lane);
