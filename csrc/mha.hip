@@ -146,21 +146,20 @@ struct Tile {
 
 // A tile of ROWS rows on its way from memory to LDS through registers: thread -> 16-byte chunk tid % CH of rows
 // tid / CH + RPI i.  Rows past the `valid` ones (at least one) repeat the last: what is computed from them is masked, and
-// holds no number that the last row did not bring in.  Columns past D repeat the first ones: they meet zeros in the other
-// operand, or are columns of a result that are not stored.  So every load is unconditional, into the register where it
-// stays until store(): nothing waits for it before.
+// holds no number that the last row did not bring in.  Columns past D are zeros: they meet zeros in the other operand (where
+// an infinity of another column would make a NaN), or are columns of a result that are not stored.  Their threads load
+// nothing and keep the zeros that their registers start with; every other load goes into the register where it stays until
+// store(): nothing waits for it before.
 template <typename T, int DP, int ROWS, int NT = THREADS>
 struct Stage {  // NT threads: the workgroup, or a wave
   static constexpr int CH = Tile<T, DP>::CH, EPC = Tile<T, DP>::EPC, RPI = NT / CH, N = ROWS / RPI;
   static_assert(ROWS % RPI == 0 && NT % CH == 0, "whole passes");
-  u32x4 r[N];
+  u32x4 r[N] = {};
   static __device__ __forceinline__ int row() { return threadIdx.x % NT / CH; }
-  static __device__ __forceinline__ int elem(int D) {
-    const int e = threadIdx.x % CH * EPC;
-    return e < D ? e : 0;
-  }
+  static __device__ __forceinline__ int elem() { return threadIdx.x % CH * EPC; }
   // p: the thread's chunk of the tile's first row; rs: elements from row to row
-  __device__ __forceinline__ void load(const T* p, long rs, int valid) {
+  __device__ __forceinline__ void load(const T* p, long rs, int valid, int D) {
+    if (elem() >= D) return;
     if (valid >= ROWS) {
       const T* q = p + row() * rs;
 #pragma unroll
@@ -172,7 +171,9 @@ struct Stage {  // NT threads: the workgroup, or a wave
   }
   // at(row of the tile): the row's address
   template <typename F>
-  __device__ __forceinline__ void gather(F&& at, int e, int valid) {
+  __device__ __forceinline__ void gather(F&& at, int valid, int D) {
+    const int e = elem();
+    if (e >= D) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const u32x4*>(at(min(row() + i * RPI, valid - 1)) + e);
   }
@@ -487,11 +488,11 @@ __global__ __launch_bounds__(THREADS, forward_waves<T>(DP)) void mha_fwd_kernel(
   load_frags<T, DP>(w.q, row < R ? at<T>(A.q, A.qs, b, t, hk * A.G + row - t * A.G) : nullptr, A.D, h);
   typedef Stage<T, DP, BN> ST;
   ST sk, sv;
-  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem(A.D);
-  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem(A.D);
+  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem();
+  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem();
   auto fetch = [&](int jt) {
-    sk.load(kp + (long)jt * BN * A.ks[1], A.ks[1], n - jt * BN);
-    sv.load(vp + (long)jt * BN * A.vs[1], A.vs[1], n - jt * BN);
+    sk.load(kp + (long)jt * BN * A.ks[1], A.ks[1], n - jt * BN, A.D);
+    sv.load(vp + (long)jt * BN * A.vs[1], A.vs[1], n - jt * BN, A.D);
   };
   if (jt1 > 0) {
     fetch(0);
@@ -559,11 +560,11 @@ __global__ __launch_bounds__(THREADS, forward_waves<T>(DP)) void mha_few_kernel(
   }
   typedef Stage<T, DP, 32, 64> ST;
   ST sk, sv;
-  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem(A.D);
-  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem(A.D);
+  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem();
+  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem();
   auto fetch = [&](int j) {
-    sk.load(kp + (long)j * 32 * A.ks[1], A.ks[1], n - j * 32);
-    sv.load(vp + (long)j * 32 * A.vs[1], A.vs[1], n - j * 32);
+    sk.load(kp + (long)j * 32 * A.ks[1], A.ks[1], n - j * 32, A.D);
+    sv.load(vp + (long)j * 32 * A.vs[1], A.vs[1], n - j * 32, A.D);
   };
   const unsigned kt = lds + wave * 2 * TILE;
   int j = split * A.split_tiles + wave;
@@ -844,11 +845,11 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dq_kernel(
   w.start(A, b, hk, tile * BM + 32 * wave + (lane & 31), n, split == 0, lane);
   typedef Stage<T, DP, BN> ST;
   ST sk, sv;
-  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem(A.D);
-  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem(A.D);
+  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem();
+  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem();
   auto fetch = [&](int jt) {
-    sk.load(kp + (long)jt * BN * A.ks[1], A.ks[1], n - jt * BN);
-    sv.load(vp + (long)jt * BN * A.vs[1], A.vs[1], n - jt * BN);
+    sk.load(kp + (long)jt * BN * A.ks[1], A.ks[1], n - jt * BN, A.D);
+    sv.load(vp + (long)jt * BN * A.vs[1], A.vs[1], n - jt * BN, A.D);
   };
   // Rows of few keys: out rounded to 16 bits, and made of weights rounded to 16, is not exact enough for a delta that
   // nearly equals dP (their gradients were off by 2.1 instead of 1.4 roundings).  Their two tiles fit into the two buffers,
@@ -941,11 +942,11 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dq_few_ker
   w.start(A, b, hk, row, n, wave == 0, lane);
   typedef Stage<T, DP, 32, 64> ST;
   ST sk, sv;
-  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem(A.D);
-  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem(A.D);
+  const T* kp = at<T>(A.k, A.ks, b, 0, hk) + ST::elem();
+  const T* vp = at<T>(A.v, A.vs, b, 0, hk) + ST::elem();
   auto fetch = [&](int j) {
-    sk.load(kp + (long)j * 32 * A.ks[1], A.ks[1], n - j * 32);
-    sv.load(vp + (long)j * 32 * A.vs[1], A.vs[1], n - j * 32);
+    sk.load(kp + (long)j * 32 * A.ks[1], A.ks[1], n - j * 32, A.D);
+    sv.load(vp + (long)j * 32 * A.vs[1], A.vs[1], n - j * 32, A.D);
   };
   const unsigned kt = lds + wave * 2 * TILE;
   int j = wave;
@@ -1111,7 +1112,7 @@ struct RowTiles {
   int st_see = 0;
 
   __device__ __forceinline__ RowTiles(const MhaArgs& A, int b, int hk, int n)
-      : A(A), b(b), hk(hk), n(n), R(A.G * A.Tq), e0(ST::elem(A.D)), per_pass(ST::RPI / A.G), me(threadIdx.x % NT),
+      : A(A), b(b), hk(hk), n(n), R(A.G * A.Tq), e0(ST::elem()), per_pass(ST::RPI / A.G), me(threadIdx.x % NT),
         blind(A.causal && A.Tq > A.Tk ? A.G * (A.Tq - A.Tk) : 0), even(ST::RPI % A.G == 0) {
     const int t0 = token_of(A, ST::row()), h0 = hk * A.G + ST::row() - t0 * A.G;
     qp = at<T>(A.q, A.qs, b, t0, h0) + e0;
@@ -1119,6 +1120,7 @@ struct RowTiles {
   }
   __device__ __forceinline__ void fetch(int it) {
     if (even && (it + 1) * BR <= R) {
+      if (e0 < A.D)
 #pragma unroll
       for (int i = 0; i < ST::N; ++i) {
         sq.r[i] = *reinterpret_cast<const u32x4*>(qp + (long)(it * ST::N + i) * (per_pass * A.qs[1]));
@@ -1129,8 +1131,8 @@ struct RowTiles {
         const int t = token_of(A, it * BR + r);
         return at<T>(p, st, b, t, hk * A.G + it * BR + r - t * A.G);
       };
-      sq.gather([&](int r) { return row_of(A.q, A.qs, r); }, e0, R - it * BR);
-      sdo.gather([&](int r) { return row_of(A.dout, A.dos, r); }, e0, R - it * BR);
+      sq.gather([&](int r) { return row_of(A.q, A.qs, r); }, R - it * BR, A.D);
+      sdo.gather([&](int r) { return row_of(A.dout, A.dos, r); }, R - it * BR, A.D);
     }
     const int row = it * BR + me;
     if (me < BR && row < R) {  // as they are: a use here would wait for every load above

@@ -104,3 +104,19 @@ def test_large_groups(tq, tk, h, hk, causal, dtype):
     q, k, v, do = make(2, tq, tk, h, hk, 32, dtype)
     lengths = [tk, tk - tk // 3]
     check(run(q, k, v, do, causal=causal, key_lengths=torch.tensor(lengths, device=DEV)), oracle(q, k, v, do, causal, lengths))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("b,tq,tk,h,hk", [(1, 1, 200, 2, 1), (2, 70, 70, 4, 2), (70, 150, 150, 4, 4)])
+@pytest.mark.parametrize("d", [8, 24, 32, 40, 56, 64, 72, 120, 128])
+def test_infinite_keys_weigh_nothing_at_every_dim(d, b, tq, tk, h, hk, dtype):
+    """An infinite element that takes a key's score to -inf gives it the weight 0, whatever the dim; its value may be
+    anything finite."""
+    q, k, v, _ = make(b, tq, tk, h, hk, d, dtype)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    shut = torch.arange(tk, device=DEV) % 5 == 2
+    k[:, shut, :, 0] = -math.inf
+    out, lse = _A().attention_forward(q, k, v)
+    want = oracle(q, k[:, ~shut], v[:, ~shut])
+    # the keys in between are in other tiles than they would be without the others: the same sums in another order
+    check({"out": out, "lse": lse}, want)
