@@ -146,10 +146,11 @@ struct Tile {
 
 // A tile of ROWS rows on its way from memory to LDS through registers: thread -> 16-byte chunk tid % CH of rows
 // tid / CH + RPI i.  Rows past the `valid` ones (at least one) repeat the last: what is computed from them is masked, and
-// holds no number that the last row did not bring in.  Columns past D are zeros: they meet zeros in the other operand (where
-// an infinity of another column would make a NaN), or are columns of a result that are not stored.  Their threads load
-// nothing and keep the zeros that their registers start with; every other load goes into the register where it stays until
-// store(): nothing waits for it before.
+// holds no number that the last row did not bring in.  Columns past D meet zeros in the other operand, or are columns of a
+// result that are not stored.  In keys and values they are zeros (an infinite element, which takes a key's weight to 0, would
+// make a NaN with a zero): their threads load nothing and keep the zeros that their registers start with.  In q and dout,
+// where an infinity is a NaN in any case, they repeat the first columns (a condition there costs the dK / dV kernel 6 %).
+// Every load goes into the register where it stays until store(): nothing waits for it before.
 template <typename T, int DP, int ROWS, int NT = THREADS>
 struct Stage {  // NT threads: the workgroup, or a wave
   static constexpr int CH = Tile<T, DP>::CH, EPC = Tile<T, DP>::EPC, RPI = NT / CH, N = ROWS / RPI;
@@ -169,13 +170,11 @@ struct Stage {  // NT threads: the workgroup, or a wave
       for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const u32x4*>(p + min(row() + i * RPI, valid - 1) * rs);
     }
   }
-  // at(row of the tile): the row's address
+  // at(row of the tile): the row's address; rows before `first` repeat it
   template <typename F>
-  __device__ __forceinline__ void gather(F&& at, int valid, int D) {
-    const int e = elem();
-    if (e >= D) return;
+  __device__ __forceinline__ void gather(F&& at, int e, int first, int valid) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const u32x4*>(at(min(row() + i * RPI, valid - 1)) + e);
+    for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const u32x4*>(at(max(first, min(row() + i * RPI, valid - 1))) + e);
   }
   __device__ __forceinline__ void store(unsigned t) const {
 #pragma unroll
@@ -1104,7 +1103,7 @@ struct RowTiles {
   typedef Stage<T, DP, BR, NT> ST;
   const MhaArgs& A;
   const int b, hk, n, R, e0, per_pass, me;
-  const int blind;  // rows in front that see no key: they are staged as zeros, whatever they hold
+  const int blind;  // rows in front that see no key: they repeat the first that sees one, as rows past the end the last
   const bool even;  // G divides the rows of a pass: a thread's rows are the same query head's, and their tokens a step apart
   const T *qp, *dop;
   ST sq, sdo;
@@ -1112,15 +1111,14 @@ struct RowTiles {
   int st_see = 0;
 
   __device__ __forceinline__ RowTiles(const MhaArgs& A, int b, int hk, int n)
-      : A(A), b(b), hk(hk), n(n), R(A.G * A.Tq), e0(ST::elem()), per_pass(ST::RPI / A.G), me(threadIdx.x % NT),
+      : A(A), b(b), hk(hk), n(n), R(A.G * A.Tq), e0(ST::elem() < A.D ? ST::elem() : 0), per_pass(ST::RPI / A.G), me(threadIdx.x % NT),
         blind(A.causal && A.Tq > A.Tk ? A.G * (A.Tq - A.Tk) : 0), even(ST::RPI % A.G == 0) {
     const int t0 = token_of(A, ST::row()), h0 = hk * A.G + ST::row() - t0 * A.G;
     qp = at<T>(A.q, A.qs, b, t0, h0) + e0;
     dop = at<T>(A.dout, A.dos, b, t0, h0) + e0;
   }
   __device__ __forceinline__ void fetch(int it) {
-    if (even && (it + 1) * BR <= R) {
-      if (e0 < A.D)
+    if (even && it * BR >= blind && (it + 1) * BR <= R) {
 #pragma unroll
       for (int i = 0; i < ST::N; ++i) {
         sq.r[i] = *reinterpret_cast<const u32x4*>(qp + (long)(it * ST::N + i) * (per_pass * A.qs[1]));
@@ -1131,8 +1129,8 @@ struct RowTiles {
         const int t = token_of(A, it * BR + r);
         return at<T>(p, st, b, t, hk * A.G + it * BR + r - t * A.G);
       };
-      sq.gather([&](int r) { return row_of(A.q, A.qs, r); }, R - it * BR, A.D);
-      sdo.gather([&](int r) { return row_of(A.dout, A.dos, r); }, R - it * BR, A.D);
+      sq.gather([&](int r) { return row_of(A.q, A.qs, r); }, e0, blind - it * BR, R - it * BR);
+      sdo.gather([&](int r) { return row_of(A.dout, A.dos, r); }, e0, blind - it * BR, R - it * BR);
     }
     const int row = it * BR + me;
     if (me < BR && row < R) {  // as they are: a use here would wait for every load above
@@ -1149,12 +1147,7 @@ struct RowTiles {
     }
   }
   // Q rows, dO rows, then L log2(e), delta, the keys each row sees; (SCALED) each row's max |dO|, the tile's
-  __device__ __forceinline__ void put(unsigned t, int it) {
-    if (it * BR < blind) {
-#pragma unroll
-      for (int i = 0; i < ST::N; ++i)
-        if (it * BR + ST::row() + i * ST::RPI < blind) sq.r[i] = sdo.r[i] = u32x4{};
-    }
+  __device__ __forceinline__ void put(unsigned t) const {
     sq.store(t);
     sdo.store(t + TILE);
     if (me < BR) {
@@ -1281,7 +1274,7 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dkv_kernel
     RowTiles<T, DP, BR, THREADS> rows(A, b, hk, n);
     if (it0 < it1) {
       rows.fetch(it0);
-      rows.put(lds, it0);
+      rows.put(lds);
     }
     mta_wait_vmem();  // the keys' operands too: a wait for them inside the loop would wait for the next tile as well
     __syncthreads();
@@ -1290,7 +1283,7 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dkv_kernel
       for (int it = from; it < to; ++it) {
         if (it + 1 < it1) rows.fetch(it + 1);
         w.template tile<BR, decltype(masked)::value>(lds + ((it - it0) & 1) * BUF, c, key, A.D, lane);
-        if (it + 1 < it1) rows.put(lds + ((it + 1 - it0) & 1) * BUF, it + 1);
+        if (it + 1 < it1) rows.put(lds + ((it + 1 - it0) & 1) * BUF);
         __syncthreads();
       }
     };
@@ -1343,7 +1336,7 @@ __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dkv_few_ke
   const unsigned qt = lds + wave * BUF;
   if (it < x.it1) rows.fetch(it);
   for (; it < x.it1; it += WAVES) {
-    rows.put(qt, it);
+    rows.put(qt);
     wave_order();
     if (it + WAVES < x.it1) rows.fetch(it + WAVES);
     if (it < x.all) w.template tile<32, true>(qt, A.scale * LOG2E, key, A.D, lane);

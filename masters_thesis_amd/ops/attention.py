@@ -201,8 +201,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, key_leng
     Query i stands at position ``i + Tk - Tq`` (the queries are the last of the sequence: a single query sees the whole
     cache).  ``causal``: it sees the keys up to its position.  ``key_lengths`` (batch,): the keys of each sequence;
     what lies behind them is never read as a number (it may be NaN) and gets zero gradients; lengths outside 0 .. Tk
-    are clamped.  (A NaN or infinity within the lengths may reach queries whose causal order hides its key.)  A query that sees no key returns 0, log-sum-exp -inf, and contributes no gradient.  ``scale``:
-    positive, default ``1 / sqrt(dim)``.
+    are clamped.  (A NaN or infinity within the lengths may reach queries whose causal order hides its key, and one in a
+    query or its output gradient the gradients of keys that are hidden from it.)  A query that sees no key returns 0,
+    log-sum-exp -inf, and contributes no gradient, whatever it and its output gradient hold.  ``scale``: positive, default
+    ``1 / sqrt(dim)``.
 
     ``return_lse``: also the log-sum-exp (batch, heads, Tq), float32, not differentiable.
 
