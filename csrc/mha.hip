@@ -1436,11 +1436,17 @@ constexpr int BLOCK = 64 * 2 / (int)sizeof(T);
 // causal, 6 of 40 58 -> 37; one head of 8192 tokens, 128 wide, 76 -> 82.
 bool few(long P, long rows) { return rows <= 32 || P * ((rows + 127) / 128) < 256; }
 // Backward: in 16 bits, where the other axis is at most 2048; a wave's own tiles of 32 keep its products less busy than
-// tiles of 64 that four share.  16 heads of 585 causal 45 -> 24 us; 2 x 1500 causal, 8 of 32 48 -> 30; 2 x 2048, 4 of 64
-// 66 -> 59; one head of 8192, 128 wide, 160 -> 294.  In fp32 the registers for both do not suffice: 3 x 777, 6 of 40 141 -> 191.
+// tiles of 64 that four share.  us in bf16 against ranges, P problems of n tokens: dim 32, 16 of 512 13 / 21, 8 of 2048
+// 39 / 49; dim 64, 16 of 585 causal 24 / 44, 8 of 1500 causal 40 / 55, 8 of 2048 62 / 67; dim 128, 16 of 585 causal 41 / 59, 8 of
+// 1024 51 / 57.  It costs where one or two problems are long (dim 64, 1 of 2048 46 / 32) and at dims past 64, one workgroup
+// on a unit, where 256 do not hold all (8 of 2048 166 / 103, 32 of 512 64 / 58).  In float16 past dim 64 the dK / dV kernel
+// spills 140 registers: short axes only there (16 of 256 32 / 37, 16 of 512 causal 48 / 71; but 16 of 64 25 / 20, 8 of
+// 1024 72 / 62, 8 of 2048 235 / 114).  In fp32 the registers for both do not suffice: 3 x 777, 6 of 40 141 -> 191.
 template <typename T>
-bool few_backward(long P, long rows, long other) {
-  return sizeof(T) == 2 && P * ((rows + 127) / 128) < 256 && other <= 2048;
+bool few_backward(long P, long rows, long other, int dp, bool causal) {
+  if (sizeof(T) != 2 || P * ((rows + 127) / 128) >= 256) return false;
+  if (SCALED<T> && dp > 64) return other <= (causal ? 512 : 256) && P * ((rows + 31) / 32) <= 256;
+  return other <= 2048;
 }
 
 // Ranges that `tiles` tiles of a sum are split into: one while `groups` workgroups fill the card, else as many as find a
@@ -1469,9 +1475,9 @@ long plan(MhaArgs& A, bool backward) {
   constexpr int BN = BLOCK<T>;
   const long kt = (A.Tk + 127) / 128;
   int per;
-  if (!few_backward<T>(P, R, A.Tk))
+  if (!few_backward<T>(P, R, A.Tk, dp, A.causal))
     ranges(P * ((R + 127) / 128), (A.Tk + BN - 1) / BN, 2, backward_waves<T>(dp), A.dq_splits, A.dq_split_tiles);
-  if (!few_backward<T>(P, A.Tk, R))
+  if (!few_backward<T>(P, A.Tk, R, dp, A.causal))
     ranges(P * (A.causal ? (kt + 1) / 2 : kt), (R + BN - 1) / BN, 4, backward_waves<T>(dp), A.kv_splits, per);
   return (A.dq_splits > 1 ? A.dq_splits * P * R * A.D : 0) + (A.kv_splits > 1 ? 2L * A.kv_splits * P * A.Tk * A.D : 0);
 }
@@ -1492,13 +1498,13 @@ int bwd(const MhaArgs& A, hipStream_t st) {
   const long R = (long)A.G * A.Tq, P = (long)A.B * A.Hkv, kt = (A.Tk + 127) / 128;
   int rc = -1;
   if constexpr (sizeof(T) == 2)
-    if (few_backward<T>(P, R, A.Tk))
+    if (few_backward<T>(P, R, A.Tk, DP, A.causal))
       rc = launch(mha_dq_few_kernel<T, DP>, grid_of(P, (R + 31) / 32), OWN > JOIN_BYTES ? OWN : JOIN_BYTES, A, st);
   if (rc < 0) rc = launch(mha_dq_kernel<T, DP, BN>, grid_of(P, (R + 127) / 128 * A.dq_splits), 4 * BN * ROW, A, st);
   if (rc) return rc;
   rc = -1;
   if constexpr (sizeof(T) == 2)
-    if (few_backward<T>(P, A.Tk, R))
+    if (few_backward<T>(P, A.Tk, R, DP, A.causal))
       rc = launch(mha_dkv_few_kernel<T, DP>, grid_of(P, (A.Tk + 31L) / 32), OWN_BUF > JOIN_BYTES ? OWN_BUF : JOIN_BYTES, A, st);
   if (rc < 0) rc = launch(mha_dkv_kernel<T, DP, BN>, grid_of(P, (A.causal ? (kt + 1) / 2 : kt) * A.kv_splits), 2 * BUF, A, st);
   if (rc) return rc;

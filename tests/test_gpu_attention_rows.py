@@ -120,3 +120,18 @@ def test_infinite_keys_weigh_nothing_at_every_dim(d, b, tq, tk, h, hk, dtype):
     want = oracle(q, k[:, ~shut], v[:, ~shut])
     # the keys in between are in other tiles than they would be without the others: the same sums in another order
     check({"out": out, "lse": lse}, want)
+
+
+@pytest.mark.parametrize("b,tq,tk,h,hk,causal,few", [(16, 200, 200, 1, 1, False, True), (8, 400, 400, 1, 1, True, True), (8, 400, 400, 1, 1, False, False),
+                                                     (2, 1000, 1000, 2, 2, True, False), (40, 300, 300, 1, 1, True, False)])
+def test_float16_kernels_of_few_problems_past_dim_64(b, tq, tk, h, hk, causal, few):
+    """Both kernels of a backward with few problems, on either side of the rule that chooses them."""
+    q, k, v, do = make(b, tq, tk, h, hk, 96, F16)
+    want = oracle(q, k, v, do, causal)
+    check(run(q, k, v, do, causal=causal), want)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        run(q, k, v, do, causal=causal)
+        torch.cuda.synchronize()
+    names = [e.key for e in prof.key_averages()]
+    assert any("mha_dkv_few_kernel" in n for n in names) == few == any("mha_dq_few_kernel" in n for n in names)
+    assert any("mha_dkv_kernel" in n for n in names) != few
