@@ -8,10 +8,12 @@ constexpr int ADAM_TABLE = 112;   // tensors of one launch: the table travels by
 // element types of a tensor and its gradient: p | g << 2
 enum { ADAM_F32 = 0, ADAM_BF16 = 1, ADAM_F16 = 2 };
 
+constexpr int ADAM_SIZE_BITS = 40;
+
 struct AdamTable {
   void* p[ADAM_TABLE];
   void* g[ADAM_TABLE];
-  long n[ADAM_TABLE];               // elements
+  uint64_t size[ADAM_TABLE];        // elements, and above ADAM_SIZE_BITS the tensor's place among the optimizer's
   unsigned block[ADAM_TABLE];       // first block of its moments
   unsigned first[ADAM_TABLE];       // first workgroup of the launch that takes it
   unsigned char type[ADAM_TABLE];
@@ -29,6 +31,8 @@ struct AdamState {
   signed char* ev;
   const float* lr;
   float* step;         // steps taken
+  float* steps;        // steps that each of the optimizer's `count` tensors has taken
+  float* factors;      // each tensor's factors of this step, four floats (see ADAM_F_*)
   double* parts;       // norm partials
   unsigned* ticket;
   float* ctl;          // this step's factors (see ADAM_CTL_*)
@@ -37,5 +41,5 @@ struct AdamState {
   uint64_t seed;
   float beta1, beta2, one_beta1, one_beta2, eps, wd;
   double dbeta1, dbeta2, dwd, max_norm, scale;
-  int decoupled, zero_grad;
+  int decoupled, zero_grad, count;
 };

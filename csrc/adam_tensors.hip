@@ -4,7 +4,9 @@
 //   p  = p (1 - lr wd, decoupled) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Two launches whatever the number of tensors (up to 112 each): the global gradient norm, whose last workgroup also
-// advances the step and derives the step's factors (without clipping: that workgroup alone), and the update.  The
+// derives the step's factors (without clipping: that workgroup alone), and the update.  t is the tensor's own count of
+// steps: one that is left out of some (no gradient) is corrected for those it took.  The factors of all tensors are
+// computed side by side from their counts, and the update's first workgroup of a tensor advances its count.  The
 // table of tensors travels by value in the kernel arguments, so a captured graph holds its own copy.
 //
 // Moments in 8 bits.  A block of 256 consecutive elements of one tensor shares a power of two 2^e, the one at or below
@@ -35,7 +37,8 @@ constexpr int WAVES = TPB / 64;
 constexpr int NORM_TPB = 512;
 constexpr int NORM_GROUPS = 256;          // workgroups of the norm at most: each ends with an add on one counter (30 ns)
 constexpr long NORM_ELEMENTS = 8192;      // and has at least so many elements
-enum { CTL_GS = 0, CTL_STEP_SIZE, CTL_BC2, CTL_DECAY, CTL_T, CTL_GS_LOW };  // gradient's factor: GS + GS_LOW
+enum { CTL_GS = 0, CTL_GS_LOW, CTL_DECAY };   // gradient's factor: GS + GS_LOW
+enum { ADAM_F_SIZE = 0, ADAM_F_BC2, ADAM_F_T };  // a tensor's step size, 1 / sqrt(1 - b2^t), t
 
 __device__ __forceinline__ float up(float x) { return x; }
 __device__ __forceinline__ float up(__bf16 x) { return (float)x; }
@@ -85,6 +88,9 @@ template <typename T>
 __device__ __forceinline__ bool aligned4(const T* p) {
   return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
 }
+
+__device__ __forceinline__ long elements(const AdamTable& t, int k) { return (long)(t.size[k] & ((1ull << ADAM_SIZE_BITS) - 1)); }
+__device__ __forceinline__ int place(const AdamTable& t, int k) { return (int)(t.size[k] >> ADAM_SIZE_BITS); }
 
 // the tensor that workgroup `g` takes
 __device__ __forceinline__ int tensor_of(const AdamTable& t, unsigned g) {
@@ -194,9 +200,17 @@ __device__ __forceinline__ double whole_power(double x, unsigned n) {
   return p;
 }
 
+// by a whole workgroup
 __device__ __forceinline__ void finish(const AdamState& s, double sq) {
-  const float t = s.step[0] + 1.f, lr = s.lr[0];
-  s.step[0] = t;
+  const float lr = s.lr[0];
+  for (int k = threadIdx.x; k < s.count; k += blockDim.x) {
+    const float t = s.steps[k] + 1.f;
+    const float size = (float)((double)lr / (1.0 - whole_power(s.dbeta1, (unsigned)t)));
+    const float bc2 = (float)(1.0 / sqrt(1.0 - whole_power(s.dbeta2, (unsigned)t)));
+    reinterpret_cast<f32x4*>(s.factors)[k] = f32x4{size, bc2, t, 0.f};
+  }
+  if (threadIdx.x != 0) return;
+  s.step[0] += 1.f;
   double gs = s.scale;
   if (s.max_norm > 0.0) {
     const double norm = sqrt(sq) * s.scale, c = s.max_norm / (norm + 1e-6);
@@ -206,15 +220,10 @@ __device__ __forceinline__ void finish(const AdamState& s, double sq) {
   }
   s.ctl[CTL_GS] = (float)gs;
   s.ctl[CTL_GS_LOW] = (float)(gs - (double)(float)gs);
-  s.ctl[CTL_STEP_SIZE] = (float)((double)lr / (1.0 - whole_power(s.dbeta1, (unsigned)t)));
-  s.ctl[CTL_BC2] = (float)(1.0 / sqrt(1.0 - whole_power(s.dbeta2, (unsigned)t)));
   s.ctl[CTL_DECAY] = s.decoupled ? (float)(1.0 - (double)lr * (double)s.wd) : 1.f;
-  s.ctl[CTL_T] = t;
 }
 
-__global__ void adam_factors_kernel(AdamState s) {
-  if (threadIdx.x == 0) finish(s, 0.0);
-}
+__global__ __launch_bounds__(NORM_TPB) void adam_factors_kernel(AdamState s) { finish(s, 0.0); }
 
 // part0: this launch's first partial; last: the list ends with this launch, whose last workgroup takes the sum
 __global__ __launch_bounds__(NORM_TPB) void adam_norm_kernel(AdamTable t, AdamState s, int part0, int nparts, int last) {
@@ -226,7 +235,7 @@ __global__ __launch_bounds__(NORM_TPB) void adam_norm_kernel(AdamTable t, AdamSt
   const unsigned end = (unsigned)((unsigned long long)t.groups * (blockIdx.x + 1) / gridDim.x);
   for (int k = tensor_of(t, w); w < end; ++k) {
     const unsigned next = min(end, k + 1 < t.count ? t.first[k + 1] : t.groups);
-    const long i0 = (long)(w - t.first[k]) * t.group, i1 = min(t.n[k], (long)(next - t.first[k]) * t.group);
+    const long i0 = (long)(w - t.first[k]) * t.group, i1 = min(elements(t, k), (long)(next - t.first[k]) * t.group);
     const int gt = t.type[k] >> 2;
     if (gt == ADAM_F32) sum += squares((const float*)t.g[k], i0, i1);
     else if (gt == ADAM_BF16) sum += squares((const __bf16*)t.g[k], i0, i1);
@@ -253,21 +262,22 @@ __global__ __launch_bounds__(NORM_TPB) void adam_norm_kernel(AdamTable t, AdamSt
   __syncthreads();
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double sq = 0.0;
-    for (int w = 0; w < NORM_TPB / 64; ++w) sq += scratch[w];
-    finish(s, sq);
-    __hip_atomic_store(s.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
+  double sq = 0.0;
+  for (int w = 0; w < NORM_TPB / 64; ++w) sq += scratch[w];
+  finish(s, sq);
+  if (threadIdx.x == 0) __hip_atomic_store(s.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---- update ------------------------------------------------------------------------------------------------------------
 template <typename P, typename G, bool WIDE, int PER>
-__device__ __forceinline__ void update(P* p, G* g, long n, unsigned block0, unsigned wg, const AdamState& s) {
+__device__ __forceinline__ void update(P* p, G* g, long n, int tensor, unsigned block0, unsigned wg, const AdamState& s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float gs = s.ctl[CTL_GS], size = s.ctl[CTL_STEP_SIZE], inv_bc2 = s.ctl[CTL_BC2], decay = s.ctl[CTL_DECAY];
+  const float gs = s.ctl[CTL_GS], decay = s.ctl[CTL_DECAY];
+  const float* f = s.factors + 4 * (long)tensor;
+  const float size = f[ADAM_F_SIZE], inv_bc2 = f[ADAM_F_BC2], taken = f[ADAM_F_T];
+  if (wg == 0 && threadIdx.x == 0) s.steps[tensor] = taken;
   const double gs64 = (double)gs + (double)s.ctl[CTL_GS_LOW];
-  const uint32_t t = (uint32_t)s.ctl[CTL_T];
+  const uint32_t t = (uint32_t)taken;
   const bool pv = aligned4(p), gv = aligned4(g);
   const long b0 = ((long)wg * WAVES + wave) * PER;  // the wave's first block of the tensor
   float pp[PER][4], gg[PER][4], mm[PER][4], vv[PER][4];
@@ -359,13 +369,14 @@ template <bool WIDE, int PER>
 __global__ __launch_bounds__(TPB) void adam_update_kernel(AdamTable t, AdamState s) {
   const int k = tensor_of(t, blockIdx.x);
   const unsigned wg = blockIdx.x - t.first[k];
-  const long n = t.n[k];
+  const long n = elements(t, k);
+  const int i = place(t, k);
   switch (t.type[k]) {
-    case ADAM_F32 | ADAM_F32 << 2: update<float, float, WIDE, PER>((float*)t.p[k], (float*)t.g[k], n, t.block[k], wg, s); break;
-    case ADAM_F32 | ADAM_BF16 << 2: update<float, __bf16, WIDE, PER>((float*)t.p[k], (__bf16*)t.g[k], n, t.block[k], wg, s); break;
-    case ADAM_F32 | ADAM_F16 << 2: update<float, _Float16, WIDE, PER>((float*)t.p[k], (_Float16*)t.g[k], n, t.block[k], wg, s); break;
-    case ADAM_BF16 | ADAM_BF16 << 2: update<__bf16, __bf16, WIDE, PER>((__bf16*)t.p[k], (__bf16*)t.g[k], n, t.block[k], wg, s); break;
-    case ADAM_F16 | ADAM_F16 << 2: update<_Float16, _Float16, WIDE, PER>((_Float16*)t.p[k], (_Float16*)t.g[k], n, t.block[k], wg, s); break;
+    case ADAM_F32 | ADAM_F32 << 2: update<float, float, WIDE, PER>((float*)t.p[k], (float*)t.g[k], n, i, t.block[k], wg, s); break;
+    case ADAM_F32 | ADAM_BF16 << 2: update<float, __bf16, WIDE, PER>((float*)t.p[k], (__bf16*)t.g[k], n, i, t.block[k], wg, s); break;
+    case ADAM_F32 | ADAM_F16 << 2: update<float, _Float16, WIDE, PER>((float*)t.p[k], (_Float16*)t.g[k], n, i, t.block[k], wg, s); break;
+    case ADAM_BF16 | ADAM_BF16 << 2: update<__bf16, __bf16, WIDE, PER>((__bf16*)t.p[k], (__bf16*)t.g[k], n, i, t.block[k], wg, s); break;
+    case ADAM_F16 | ADAM_F16 << 2: update<_Float16, _Float16, WIDE, PER>((_Float16*)t.p[k], (_Float16*)t.g[k], n, i, t.block[k], wg, s); break;
   }
 }
 
@@ -448,7 +459,7 @@ extern "C" void mta_adam_tensors(const AdamTable* tables, int count, const AdamS
       part0 += parts;
     }
   } else {
-    adam_factors_kernel<<<1, 64, 0, st>>>(*s);
+    adam_factors_kernel<<<1, NORM_TPB, 0, st>>>(*s);
   }
   for (int k = 0; k < count; ++k) {
     const bool few = tables[k].group == 4 * ADAM_BLOCK;

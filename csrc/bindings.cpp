@@ -1339,12 +1339,16 @@ AdamState adam_state(const std::vector<at::Tensor>& state, int64_t blocks) {
   return s;
 }
 
-// control: float32 [factors 8 | step | lr | grad norm | non-finite norms], parts: float64, ticket: int32 (zero)
+// params, grads and, of each, its first block of moments and its place among the optimizer's tensors; lr, step, norm,
+// nonfinite: one float32 each, steps: one for each of the optimizer's tensors, ctl: 8 and 4 for each of them (factors of the
+// step); parts: float64, ticket: int32 (zero)
 void adam_tensors(std::vector<at::Tensor> params, std::vector<at::Tensor> grads, std::vector<int64_t> blocks,
-                  std::vector<at::Tensor> state, at::Tensor lr, at::Tensor step, at::Tensor ctl, at::Tensor norm,
+                  std::vector<int64_t> places, std::vector<at::Tensor> state, at::Tensor lr, at::Tensor step, at::Tensor steps,
+                  at::Tensor ctl, at::Tensor norm,
                   at::Tensor nonfinite, at::Tensor parts, at::Tensor ticket, double beta1, double beta2, double eps, double wd,
                   double max_norm, double scale, bool adamw, bool zero_grad, int64_t seed) {
-  TORCH_CHECK(params.size() == grads.size() && params.size() == blocks.size(), "adam_tensors: lists of one length");
+  TORCH_CHECK(params.size() == grads.size() && params.size() == blocks.size() && params.size() == places.size(),
+              "adam_tensors: lists of one length");
   TORCH_CHECK(!state.empty(), "adam_tensors: no state");
   const auto device = state[0].device();
   int64_t end = 0, elements = 0;
@@ -1369,10 +1373,12 @@ void adam_tensors(std::vector<at::Tensor> params, std::vector<at::Tensor> grads,
       tables.back().groups = 0;
     }
     AdamTable& t = tables.back();
-    TORCH_CHECK(groups <= 0x7fffffffL, "adam_tensors: tensor ", i, " is too large");
+    TORCH_CHECK(groups <= 0x7fffffffL && n < 1L << ADAM_SIZE_BITS, "adam_tensors: tensor ", i, " is too large");
+    TORCH_CHECK(places[i] >= 0 && places[i] < steps.numel() && places[i] < 1L << (64 - ADAM_SIZE_BITS),
+                "adam_tensors: place of tensor ", i);
     t.p[t.count] = p.data_ptr();
     t.g[t.count] = g.data_ptr();
-    t.n[t.count] = n;
+    t.size[t.count] = (uint64_t)n | (uint64_t)places[i] << ADAM_SIZE_BITS;
     t.block[t.count] = (unsigned)blocks[i];
     t.first[t.count] = t.groups;
     t.type[t.count] = (unsigned char)(pt | gt << 2);
@@ -1388,9 +1394,9 @@ void adam_tensors(std::vector<at::Tensor> params, std::vector<at::Tensor> grads,
       TORCH_CHECK(spans[i].first >= spans[i - 1].second, "adam_tensors: gradients that are to be zeroed share memory");
   }
   AdamState s = adam_state(state, end);
-  for (const at::Tensor* t : {&lr, &step, &norm, &nonfinite, &ctl}) {
+  for (const at::Tensor* t : {&lr, &step, &norm, &nonfinite, &steps, &ctl}) {
     CHECK_F32(*t);
-    TORCH_CHECK(t->device() == device && t->numel() >= (t == &ctl ? 8 : 1), "adam_tensors: control buffers");
+    TORCH_CHECK(t->device() == device && t->numel() >= (t == &ctl ? 8 + 4 * steps.numel() : 1), "adam_tensors: control buffers");
   }
   TORCH_CHECK(parts.device() == device && parts.scalar_type() == at::kDouble && parts.is_contiguous() &&
                   parts.numel() >= (int64_t)std::max<size_t>(tables.size(), 1) * mta_adam_norm_parts(),
@@ -1399,7 +1405,10 @@ void adam_tensors(std::vector<at::Tensor> params, std::vector<at::Tensor> grads,
   if (tables.empty()) return;
   s.lr = lr.data_ptr<float>();
   s.step = step.data_ptr<float>();
+  s.steps = steps.data_ptr<float>();
+  s.count = (int)steps.numel();
   s.ctl = ctl.data_ptr<float>();
+  s.factors = s.ctl + 8;
   s.norm = norm.data_ptr<float>();
   s.nonfinite = nonfinite.data_ptr<float>();
   s.parts = parts.data_ptr<double>();

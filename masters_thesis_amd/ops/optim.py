@@ -302,9 +302,9 @@ _BLOCK = 256  # csrc/adam_tensors.h ADAM_BLOCK: elements of a tensor that share 
 _M32 = 0xFFFFFFFF
 
 
-def _chances(seed: int, step: int, n: int, device) -> tuple:
-    """Two 16-bit random numbers for each of n elements (csrc/adam_tensors.hip chance_of)."""
-    i = torch.arange(n, device=device)
+def _chances(seed: int, step: int, n: int, device, first: int = 0) -> tuple:
+    """Two 16-bit random numbers for each of n elements from ``first`` on (csrc/adam_tensors.hip chance_of)."""
+    i = torch.arange(first, first + n, device=device)
     x = (seed & _M32) ^ ((step * 0x9E3779B1) & _M32) ^ (((seed >> 32) * 0x85EBCA77) & _M32)
     x = ((i >> 32) * 0x27D4EB2F) & _M32 ^ (i & _M32) ^ x
     x = ((x ^ (x >> 16)) * 0x7FEB352D) & _M32
@@ -355,7 +355,8 @@ class TensorAdam:
     parameter instead of 8.  A NaN or infinite gradient makes the moments of its block NaN.
 
     ``step(grads=...)`` takes the gradients in the parameters' order; without it, ``p.grad``.  A parameter whose
-    gradient is None is left out of the step.  Gradients are not changed unless ``zero_grad`` is set.
+    gradient is None is left out of the step: each tensor has its own count of steps (``steps``), as in torch.optim.
+    Gradients are not changed unless ``zero_grad`` is set.
     """
 
     def __init__(self, params: Iterable[Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -394,7 +395,9 @@ class TensorAdam:
             self._state = [torch.zeros(at, device=dev, dtype=torch.uint8) for _ in range(2)]
             self._state += [torch.full((at // _BLOCK,), -100, device=dev, dtype=torch.int8) for _ in range(2)]
         self.lr_t = torch.tensor([lr], **f32)
+        #: steps taken, and by each tensor
         self.step_t = torch.zeros(1, **f32)
+        self.steps = torch.zeros(len(self.params), **f32)
         #: norm of the last step's scaled gradient, and the count of steps where it was not finite: with ``max_norm`` only
         self.grad_norm = torch.zeros(1, **f32)
         self.nonfinite = torch.zeros(1, **f32)
@@ -406,7 +409,7 @@ class TensorAdam:
             launches = -(-len(self.params) // C.ADAM_TABLE) + sum(p.numel() >> 42 for p in self.params)
             self._parts = torch.zeros(launches * C.adam_norm_parts(), device=dev, dtype=torch.float64)
             self._ticket = torch.zeros(1, device=dev, dtype=torch.int32)
-            self._ctl = torch.zeros(8, **f32)
+            self._ctl = torch.zeros(8 + 4 * len(self.params), **f32)
         self.param_groups = [{
             "lr": lr, "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay, "amsgrad": False,
             "maximize": False, "foreach": None, "capturable": True, "differentiable": False, "fused": True,
@@ -437,26 +440,26 @@ class TensorAdam:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdam: {len(grads)} gradients for {len(self.params)} parameters")
-        params, blocks = self.params, self._blocks if self.hip else self.offsets
+        params, blocks, places = self.params, self._blocks if self.hip else self.offsets, list(range(len(grads)))
         if any(g is None for g in grads):
-            keep = [i for i, g in enumerate(grads) if g is not None]
-            params, blocks, grads = [params[i] for i in keep], [blocks[i] for i in keep], [grads[i] for i in keep]
+            places = [i for i, g in enumerate(grads) if g is not None]
+            params, blocks, grads = [params[i] for i in places], [blocks[i] for i in places], [grads[i] for i in places]
         if not grads:
             return
         if not self.hip:
-            self._step_torch(params, blocks, grads, max_norm, grad_scale)
+            self._step_torch(params, blocks, places, grads, max_norm, grad_scale)
             if zero_grad:
                 for g in grads:
                     g.zero_()
         else:
             if not zero_grad:
                 grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-            lib().adam_tensors(params, grads, blocks, self._state, self.lr_t, self.step_t, self._ctl, self.grad_norm,
-                               self.nonfinite, self._parts, self._ticket, *self.betas, self.eps, self.weight_decay,
+            lib().adam_tensors(params, grads, blocks, places, self._state, self.lr_t, self.step_t, self.steps, self._ctl,
+                               self.grad_norm, self.nonfinite, self._parts, self._ticket, *self.betas, self.eps, self.weight_decay,
                                float(max_norm or 0.0), float(grad_scale), self.adamw, bool(zero_grad), self.seed)
         self.grads_zeroed = bool(zero_grad)
 
-    def _step_torch(self, params, offsets, grads, max_norm, grad_scale) -> None:
+    def _step_torch(self, params, offsets, places, grads, max_norm, grad_scale) -> None:
         b1, b2 = self.betas
         scale = float(grad_scale)
         if max_norm and max_norm > 0:
@@ -466,15 +469,20 @@ class TensorAdam:
                 self.nonfinite += 1
             scale = scale * torch.clamp(max_norm / (norm + 1e-6), max=1.0)
         self.step_t += 1
-        t = int(self.step_t.item())
         m, v = self.moments()
         kind = torch.float32
         if self.state_bits == 8:  # up to their rounding in 64 bits, as csrc/adam_tensors.hip
             kind, m, v = torch.float64, m.double(), v.double()
-        for p, g, o in zip(params, grads, offsets):
+        chances = torch.zeros(2, self.padded if self.state_bits == 8 else 0, dtype=torch.long, device=m.device)
+        took = torch.zeros(self.padded // _BLOCK, dtype=torch.bool, device=m.device)
+        for p, g, o, place in zip(params, grads, offsets, places):
             if p.shape != g.shape:
                 raise ValueError(f"TensorAdam: parameter {tuple(p.shape)} with gradient {tuple(g.shape)}")
             n = p.numel()
+            if not n:
+                continue
+            self.steps[place] += 1
+            t = int(self.steps[place].item())
             x, gg, mm, vv = p.float().reshape(-1), g.to(kind).reshape(-1) * scale, m[o:o + n], v[o:o + n]
             if not self.adamw:
                 gg = gg + x.to(kind) * self.weight_decay
@@ -483,12 +491,12 @@ class TensorAdam:
             x = x * (1 - self._lr * self.weight_decay) if self.adamw else x
             x = x - mm.float() / (vv.float().sqrt() / math.sqrt(1 - b2 ** t) + self.eps) * (self._lr / (1 - b1 ** t))
             p.copy_(x.view(p.shape))
+            if self.state_bits == 8:
+                end = o + -(-n // _BLOCK) * _BLOCK
+                took[o // _BLOCK:end // _BLOCK] = True
+                chances[0, o:end], chances[1, o:end] = _chances(self.seed, t, end - o, m.device, o)
         if self.state_bits == 8:
-            low, high = _chances(self.seed, t, self.padded, m.device)
-            took = torch.zeros(self.padded // _BLOCK, dtype=torch.bool, device=m.device)
-            for p, o in zip(params, offsets):
-                took[o // _BLOCK:(o + p.numel() + _BLOCK - 1) // _BLOCK] = True
-            self._put8(m, v, low, high, took)
+            self._put8(m, v, chances[0], chances[1], took)
 
     def _put8(self, m, v, low, high, took, loaded: bool = False) -> None:
         mc, me = _encode8(m, low, 3, loaded)
@@ -521,9 +529,9 @@ class TensorAdam:
         return [buf[o:o + p.numel()].view(p.shape) for p, o in zip(self.params, self.offsets)]
 
     def state_dict(self) -> Dict:
-        step = self.step_t.detach().cpu().reshape(())
+        steps = self.steps.detach().cpu()
         m, v = self.moments()
-        state = {i: {"step": step.clone(), "exp_avg": a.detach().cpu().clone(), "exp_avg_sq": b.detach().cpu().clone()}
+        state = {i: {"step": steps[i].clone(), "exp_avg": a.detach().cpu().clone(), "exp_avg_sq": b.detach().cpu().clone()}
                  for i, (a, b) in enumerate(zip(self._views(m), self._views(v)))}
         return {"state": state, "param_groups": [dict(self.param_groups[0])]}
 
@@ -538,12 +546,13 @@ class TensorAdam:
         self.set_lr(g["lr"])
         m, v = self.moments()
         mvs, vvs = self._views(m), self._views(v)
-        step = 0.0
+        steps = [0.0] * len(self.params)
         for i, st in sd["state"].items():
             mvs[int(i)].copy_(st["exp_avg"].reshape(mvs[int(i)].shape))
             vvs[int(i)].copy_(st["exp_avg_sq"].reshape(vvs[int(i)].shape))
-            step = float(st["step"])
-        self.step_t.fill_(step)
+            steps[int(i)] = float(st["step"])
+        self.steps.copy_(torch.tensor(steps))
+        self.step_t.fill_(max(steps))
         if self.state_bits == 8:
             if self.hip:
                 lib().adam_moments(self._state, m, v, False)

@@ -1,0 +1,64 @@
+"""ops.optim.TensorAdam on the GPU: tensors that start late or are left out of steps."""
+import pytest
+import torch
+
+from test_tensor_adam_steps_cpu import SHAPES, run, tensors
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("adamw", [True, False])
+def test_each_tensor_has_its_own_steps(adamw):
+    opt, ref, off = run(32, adamw, DEV)
+    assert off <= 12 * (32 * 0.1 * 2.0 ** -22 + 4 * 2.0 ** -23)  # as on the CPU
+    mine, its = opt.state_dict()["state"], ref.state_dict()["state"]
+    assert [float(mine[i]["step"]) for i in range(3)] == [float(its[i]["step"]) for i in range(3)] and float(opt.step_t) == opt.calls
+
+
+def test_codes_of_left_out_tensors_are_the_cpus():
+    a, _, _ = run(8, True, DEV)
+    b, _, _ = run(8, True)
+    assert all(torch.equal(x.cpu(), y) for x, y in zip(a._state, b._state)) and torch.equal(a.steps.cpu(), b.steps)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_tensors_than_a_launch_takes(bits):
+    """Counts and factors of every tensor, in whichever launch it is, with and without clipping; empty tensors between."""
+    from masters_thesis_amd.ops.optim import TensorAdam
+
+    n = 300
+    shapes = [(0,) if i % 50 == 7 else (1 + 37 * i % 700,) for i in range(n)]
+    ps, qs = [p.to(DEV) for p in tensors(shapes)], tensors(shapes)
+    a, b = TensorAdam(ps, lr=1e-2, state_bits=bits), TensorAdam(qs, lr=1e-2, state_bits=bits)
+    for t in range(4):
+        gs = [g if (i + t) % 3 or t == 3 else None for i, g in enumerate(tensors(shapes, seed=t + 1))]
+        norm = 1.0 if t % 2 else 0.0
+        a.step(max_norm=norm, grads=[None if g is None else g.to(DEV) for g in gs])
+        b.step(max_norm=norm, grads=gs)
+        assert torch.equal(a.steps.cpu(), b.steps)
+    for p, q in zip(ps, qs):
+        assert torch.allclose(p.cpu(), q, rtol=1e-5, atol=1e-6)
+
+
+def test_captured_steps_count_for_the_tensors_they_take():
+    from masters_thesis_amd.ops.optim import TensorAdam
+
+    ps, qs = [p.to(DEV) for p in tensors(SHAPES)], [p.to(DEV) for p in tensors(SHAPES)]
+    gs = [g.to(DEV) for g in tensors(SHAPES, seed=1)]
+    a, b = (TensorAdam(x, lr=1e-2, state_bits=8) for x in (ps, qs))
+    for o in (a, b):
+        o.step(1.0, grads=gs)
+    part = [gs[0], None, gs[2]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(1.0, grads=part)
+    for t in range(3):
+        graph.replay()
+        b.step(1.0, grads=part)
+        if t == 1:
+            for o in (a, b):
+                o.step(grads=gs)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(ps + a._state, qs + b._state)) and torch.equal(a.steps, b.steps)
+    assert a.steps.tolist() == [5.0, 2.0, 5.0]

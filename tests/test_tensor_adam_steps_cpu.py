@@ -1,0 +1,63 @@
+"""ops.optim.TensorAdam: tensors that start late or are left out, and states of part of the tensors, as torch.optim has them."""
+import pytest
+import torch
+
+from masters_thesis_amd.ops.optim import TensorAdam
+
+
+def tensors(shapes, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g) for s in shapes]
+
+
+SHAPES = [(300,), (7, 5), (260,)]
+
+
+def run(state_bits, adamw, device="cpu", steps=12):
+    """The optimizer and torch's on the same gradients, some left out: the largest difference of the parameters."""
+    ps = [p.to(device) for p in tensors(SHAPES)]
+    qs = [torch.nn.Parameter(p.clone()) for p in tensors(SHAPES)]
+    opt = TensorAdam(ps, lr=0.1, betas=(0.9, 0.99), weight_decay=0.01, adamw=adamw, state_bits=state_bits)
+    ref = (torch.optim.AdamW if adamw else torch.optim.Adam)(qs, lr=0.1, betas=(0.9, 0.99), weight_decay=0.01)
+    opt.calls = 0
+    for t in range(steps):
+        gs = [g if (t + i) % (i + 2) == 0 or t > 8 else None for i, g in enumerate(tensors(SHAPES, seed=t + 1))]
+        if t < 5:
+            gs[2] = None  # starts late
+        for q, g in zip(qs, gs):
+            q.grad = g
+        ref.step()
+        opt.calls += any(g is not None for g in gs)
+        opt.step(grads=[None if g is None else g.to(device) for g in gs])
+    return opt, ref, max(float((p.cpu() - q.detach()).abs().max()) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("adamw", [True, False])
+def test_each_tensor_has_its_own_steps(adamw):
+    opt, ref, off = run(32, adamw)
+    # 12 updates of at most about lr * 3.2 of some 20 fp32 operations each, on parameters up to 4
+    assert off <= 12 * (32 * 0.1 * 2.0 ** -22 + 4 * 2.0 ** -23)
+    mine, its = opt.state_dict()["state"], ref.state_dict()["state"]
+    assert [float(mine[i]["step"]) for i in range(3)] == [float(its[i]["step"]) for i in range(3)] and float(opt.step_t) == opt.calls
+
+
+def test_a_late_tensor_moves_as_a_first_step():
+    ps = [torch.zeros(4), torch.zeros(4)]
+    opt = TensorAdam(ps, lr=1.0, weight_decay=0.0)
+    for _ in range(50):
+        opt.step(grads=[torch.ones(4), None])
+    opt.step(grads=[None, torch.ones(4)])
+    assert torch.allclose(ps[1], torch.full((4,), -1.0), rtol=1e-6)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_steps_of_a_state_load_tensor_by_tensor(bits):
+    a, _, _ = run(bits, True)
+    b = TensorAdam([p.clone() for p in a.params], lr=0.3, state_bits=bits)
+    b.load_state_dict(a.state_dict())
+    assert torch.equal(a.steps, b.steps) and len(set(a.steps.tolist())) > 1
+    for t in range(3):
+        for o in (a, b):
+            o.step(grads=tensors(SHAPES, seed=90 + t))
+    assert all(torch.equal(x, y) for x, y in zip(a.params, b.params))
+    assert all(torch.equal(x, y) for x, y in zip(a._state, b._state))
