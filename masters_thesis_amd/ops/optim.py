@@ -537,7 +537,8 @@ class TensorAdam:
 
     @torch.no_grad()
     def load_state_dict(self, sd: Dict) -> None:
-        """Moments go to the nearest code in 8 bits (a state of this optimizer's own: to the values it had)."""
+        """Moments go to the nearest code in 8 bits (a state of this optimizer's own: to the values it had).  Tensors that
+        the state has no entry of start anew."""
         g = sd["param_groups"][0]
         self.betas = tuple(float(b) for b in g.get("betas", self.betas))
         self.eps = float(g.get("eps", self.eps))
@@ -547,6 +548,8 @@ class TensorAdam:
         m, v = self.moments()
         mvs, vvs = self._views(m), self._views(v)
         steps = [0.0] * len(self.params)
+        for i in set(range(len(self.params))) - {int(i) for i in sd["state"]}:
+            mvs[i].zero_(), vvs[i].zero_()
         for i, st in sd["state"].items():
             mvs[int(i)].copy_(st["exp_avg"].reshape(mvs[int(i)].shape))
             vvs[int(i)].copy_(st["exp_avg_sq"].reshape(vvs[int(i)].shape))

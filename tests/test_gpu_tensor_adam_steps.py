@@ -62,3 +62,15 @@ def test_captured_steps_count_for_the_tensors_they_take():
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(ps + a._state, qs + b._state)) and torch.equal(a.steps, b.steps)
     assert a.steps.tolist() == [5.0, 2.0, 5.0]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_loaded_state_replaces_all_moments(bits):
+    a, _, _ = run(bits, True, DEV)
+    full = a.state_dict()
+    a.load_state_dict({"state": {1: full["state"][1]}, "param_groups": full["param_groups"]})
+    m, v = a.moments()
+    o, n = a.offsets[1], a.params[1].numel()
+    assert torch.equal(m[o:o + n].cpu(), full["state"][1]["exp_avg"].view(-1)) and m[o:o + n].any()
+    m[o:o + n] = v[o:o + n] = 0
+    assert not m.any() and not v.any() and a.steps.tolist() == [0.0, float(full["state"][1]["step"]), 0.0]

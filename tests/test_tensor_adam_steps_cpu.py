@@ -61,3 +61,23 @@ def test_steps_of_a_state_load_tensor_by_tensor(bits):
             o.step(grads=tensors(SHAPES, seed=90 + t))
     assert all(torch.equal(x, y) for x, y in zip(a.params, b.params))
     assert all(torch.equal(x, y) for x, y in zip(a._state, b._state))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_loaded_state_replaces_all_moments(bits):
+    """Tensors without an entry start anew, as in torch.optim: an empty state, then one of a single tensor."""
+    a, _, _ = run(bits, True)
+    full = a.state_dict()
+    for keep in ([], [1]):
+        b, _, _ = run(bits, True)
+        b.load_state_dict({"state": {i: full["state"][i] for i in keep}, "param_groups": full["param_groups"]})
+        m, v = b.moments()
+        for i, (o, p) in enumerate(zip(b.offsets, b.params)):
+            if i in keep:
+                assert torch.equal(m[o:o + p.numel()].view(p.shape), full["state"][i]["exp_avg"]) and b.steps[i] == full["state"][i]["step"]
+            else:
+                assert not m[o:o + p.numel()].any() and not v[o:o + p.numel()].any() and b.steps[i] == 0
+        fresh = TensorAdam([p.clone() for p in b.params], lr=b.lr, betas=b.betas, weight_decay=b.weight_decay, state_bits=bits)
+        gs = tensors(SHAPES, seed=70)
+        b.step(grads=gs), fresh.step(grads=gs)
+        assert all(torch.equal(x, y) for i, (x, y) in enumerate(zip(b.params, fresh.params)) if i not in keep)
