@@ -8,16 +8,15 @@ constexpr int ADAM_TABLE = 112;   // tensors of one launch: the table travels by
 // element types of a tensor and its gradient: p | g << 2
 enum { ADAM_F32 = 0, ADAM_BF16 = 1, ADAM_F16 = 2 };
 
-constexpr int ADAM_SIZE_BITS = 40;
-
 struct AdamTable {
   void* p[ADAM_TABLE];
   void* g[ADAM_TABLE];
-  uint64_t size[ADAM_TABLE];        // elements, and above ADAM_SIZE_BITS the tensor's place among the optimizer's
+  long n[ADAM_TABLE];               // elements; 0 for a tensor that is left out of the step
   unsigned block[ADAM_TABLE];       // first block of its moments
   unsigned first[ADAM_TABLE];       // first workgroup of the launch that takes it
   unsigned char type[ADAM_TABLE];
   int count;
+  int place;                        // of the table's first tensor among the optimizer's
   int group;                        // elements of a workgroup
   unsigned groups;                  // workgroups over all tensors
 };
@@ -42,4 +41,5 @@ struct AdamState {
   float beta1, beta2, one_beta1, one_beta2, eps, wd;
   double dbeta1, dbeta2, dwd, max_norm, scale;
   int decoupled, zero_grad, count;
+  int skip;            // a step whose gradient norm is not finite changes nothing (the norm is taken without clipping too)
 };

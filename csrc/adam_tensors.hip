@@ -37,7 +37,7 @@ constexpr int WAVES = TPB / 64;
 constexpr int NORM_TPB = 512;
 constexpr int NORM_GROUPS = 256;          // workgroups of the norm at most: each ends with an add on one counter (30 ns)
 constexpr long NORM_ELEMENTS = 8192;      // and has at least so many elements
-enum { CTL_GS = 0, CTL_GS_LOW, CTL_DECAY };   // gradient's factor: GS + GS_LOW
+enum { CTL_GS = 0, CTL_GS_LOW, CTL_DECAY, CTL_SKIP };  // gradient's factor: GS + GS_LOW; SKIP: this step changes nothing
 enum { ADAM_F_SIZE = 0, ADAM_F_BC2, ADAM_F_T };  // a tensor's step size, 1 / sqrt(1 - b2^t), t
 
 __device__ __forceinline__ float up(float x) { return x; }
@@ -89,10 +89,7 @@ __device__ __forceinline__ bool aligned4(const T* p) {
   return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
 }
 
-__device__ __forceinline__ long elements(const AdamTable& t, int k) { return (long)(t.size[k] & ((1ull << ADAM_SIZE_BITS) - 1)); }
-__device__ __forceinline__ int place(const AdamTable& t, int k) { return (int)(t.size[k] >> ADAM_SIZE_BITS); }
-
-// the tensor that workgroup `g` takes
+// the tensor that workgroup `g` takes: the last that starts at or before it, so never an empty one
 __device__ __forceinline__ int tensor_of(const AdamTable& t, unsigned g) {
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
@@ -200,23 +197,28 @@ __device__ __forceinline__ double whole_power(double x, unsigned n) {
   return p;
 }
 
-// by a whole workgroup
+// by a whole workgroup: the tensors' factors by all waves but the first, whose first thread takes what they share
 __device__ __forceinline__ void finish(const AdamState& s, double sq) {
   const float lr = s.lr[0];
-  for (int k = threadIdx.x; k < s.count; k += blockDim.x) {
+  for (int k = (int)threadIdx.x - 64; k >= 0 && k < s.count; k += NORM_TPB - 64) {
     const float t = s.steps[k] + 1.f;
     const float size = (float)((double)lr / (1.0 - whole_power(s.dbeta1, (unsigned)t)));
     const float bc2 = (float)(1.0 / sqrt(1.0 - whole_power(s.dbeta2, (unsigned)t)));
     reinterpret_cast<f32x4*>(s.factors)[k] = f32x4{size, bc2, t, 0.f};
   }
   if (threadIdx.x != 0) return;
-  s.step[0] += 1.f;
+  const double norm = sqrt(sq) * s.scale;
+  const bool bad = !isfinite((float)norm), skip = s.skip && bad;
+  if (s.max_norm > 0.0 || s.skip) {
+    s.norm[0] = (float)norm;
+    if (bad) s.nonfinite[0] += 1.f;
+  }
+  s.ctl[CTL_SKIP] = skip ? 1.f : 0.f;
+  if (!skip) s.step[0] += 1.f;
   double gs = s.scale;
   if (s.max_norm > 0.0) {
-    const double norm = sqrt(sq) * s.scale, c = s.max_norm / (norm + 1e-6);
-    s.norm[0] = (float)norm;
-    if (!isfinite((float)norm)) s.nonfinite[0] += 1.f;
-    gs *= c < 1.0 ? c : (c != c ? c : 1.0);  // a NaN norm stays visible
+    const double c = s.max_norm / (norm + 1e-6);
+    gs *= c < 1.0 ? c : (c != c ? c : 1.0);  // a NaN norm stays visible (as torch's clipping), unless skipped
   }
   s.ctl[CTL_GS] = (float)gs;
   s.ctl[CTL_GS_LOW] = (float)(gs - (double)(float)gs);
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(NORM_TPB) void adam_norm_kernel(AdamTable t, AdamSt
   const unsigned end = (unsigned)((unsigned long long)t.groups * (blockIdx.x + 1) / gridDim.x);
   for (int k = tensor_of(t, w); w < end; ++k) {
     const unsigned next = min(end, k + 1 < t.count ? t.first[k + 1] : t.groups);
-    const long i0 = (long)(w - t.first[k]) * t.group, i1 = min(elements(t, k), (long)(next - t.first[k]) * t.group);
+    const long i0 = (long)(w - t.first[k]) * t.group, i1 = min(t.n[k], (long)(next - t.first[k]) * t.group);
     const int gt = t.type[k] >> 2;
     if (gt == ADAM_F32) sum += squares((const float*)t.g[k], i0, i1);
     else if (gt == ADAM_BF16) sum += squares((const __bf16*)t.g[k], i0, i1);
@@ -275,7 +277,7 @@ __device__ __forceinline__ void update(P* p, G* g, long n, int tensor, unsigned 
   const float gs = s.ctl[CTL_GS], decay = s.ctl[CTL_DECAY];
   const float* f = s.factors + 4 * (long)tensor;
   const float size = f[ADAM_F_SIZE], inv_bc2 = f[ADAM_F_BC2], taken = f[ADAM_F_T];
-  if (wg == 0 && threadIdx.x == 0) s.steps[tensor] = taken;
+  const bool skip = s.ctl[CTL_SKIP] != 0.f;  // asked for with all loads on their way, which would wait for it otherwise
   const double gs64 = (double)gs + (double)s.ctl[CTL_GS_LOW];
   const uint32_t t = (uint32_t)taken;
   const bool pv = aligned4(p), gv = aligned4(g);
@@ -287,8 +289,15 @@ __device__ __forceinline__ void update(P* p, G* g, long n, int tensor, unsigned 
   for (int u = 0; u < PER; ++u) {
     const long i = (b0 + u) * ADAM_BLOCK + lane * 4;
     if ((b0 + u) * ADAM_BLOCK >= n) continue;
-    load4(p, i, n, pv, pp[u]);
-    load4(g, i, n, gv, gg[u]);
+    // whole blocks by all lanes at once: with the other way's loads into the same registers in between, each waits for the last
+    const bool whole = (b0 + u + 1) * ADAM_BLOCK <= n;
+    if (__builtin_amdgcn_readfirstlane(whole && pv && gv)) {
+      load4(p, i, i + 4, true, pp[u]);
+      load4(g, i, i + 4, true, gg[u]);
+    } else {
+      load4(p, i, n, pv, pp[u]);
+      load4(g, i, n, gv, gg[u]);
+    }
     const long sb = (long)block0 + b0 + u, si = sb * ADAM_BLOCK + lane * 4;  // the state is padded to whole blocks
     if constexpr (WIDE) {
       const f32x4 a = *reinterpret_cast<const f32x4*>(s.m32 + si), b = *reinterpret_cast<const f32x4*>(s.v32 + si);
@@ -304,6 +313,13 @@ __device__ __forceinline__ void update(P* p, G* g, long n, int tensor, unsigned 
       ev[u] = s.ev[sb];
     }
   }
+  if (skip) {
+    if (!s.zero_grad) return;
+#pragma unroll 1
+    for (int u = 0; u < PER; ++u) store4(g, (b0 + u) * ADAM_BLOCK + lane * 4, n, gv, {0.f, 0.f, 0.f, 0.f});
+    return;
+  }
+  if (wg == 0 && threadIdx.x == 0) s.steps[tensor] = taken;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const long i = (b0 + u) * ADAM_BLOCK + lane * 4;
@@ -369,8 +385,8 @@ template <bool WIDE, int PER>
 __global__ __launch_bounds__(TPB) void adam_update_kernel(AdamTable t, AdamState s) {
   const int k = tensor_of(t, blockIdx.x);
   const unsigned wg = blockIdx.x - t.first[k];
-  const long n = elements(t, k);
-  const int i = place(t, k);
+  const long n = t.n[k];
+  const int i = t.place + k;
   switch (t.type[k]) {
     case ADAM_F32 | ADAM_F32 << 2: update<float, float, WIDE, PER>((float*)t.p[k], (float*)t.g[k], n, i, t.block[k], wg, s); break;
     case ADAM_F32 | ADAM_BF16 << 2: update<float, __bf16, WIDE, PER>((float*)t.p[k], (__bf16*)t.g[k], n, i, t.block[k], wg, s); break;
@@ -448,9 +464,9 @@ inline int grid_blocks(long blocks) {
 extern "C" int mta_adam_group(long elements) { return elements < (4L << 20) ? 4 * ADAM_BLOCK : 16 * ADAM_BLOCK; }
 extern "C" int mta_adam_norm_parts() { return NORM_GROUPS; }
 
-// tables: `count` of them.  The norm over all of them first (clip on), then the update of each.
+// tables: `count` of them.  The norm over all of them first (with clipping or skipping), then the update of each.
 extern "C" void mta_adam_tensors(const AdamTable* tables, int count, const AdamState* s, int wide, hipStream_t st) {
-  if (s->max_norm > 0.0) {
+  if (s->max_norm > 0.0 || s->skip) {
     int part0 = 0;
     for (int k = 0; k < count; ++k) {
       const long want = ((long)tables[k].groups * tables[k].group + NORM_ELEMENTS - 1) / NORM_ELEMENTS;

@@ -1339,56 +1339,60 @@ AdamState adam_state(const std::vector<at::Tensor>& state, int64_t blocks) {
   return s;
 }
 
-// params, grads and, of each, its first block of moments and its place among the optimizer's tensors; lr, step, norm,
-// nonfinite: one float32 each, steps: one for each of the optimizer's tensors, ctl: 8 and 4 for each of them (factors of the
-// step); parts: float64, ticket: int32 (zero)
-void adam_tensors(std::vector<at::Tensor> params, std::vector<at::Tensor> grads, std::vector<int64_t> blocks,
-                  std::vector<int64_t> places, std::vector<at::Tensor> state, at::Tensor lr, at::Tensor step, at::Tensor steps,
-                  at::Tensor ctl, at::Tensor norm,
-                  at::Tensor nonfinite, at::Tensor parts, at::Tensor ticket, double beta1, double beta2, double eps, double wd,
-                  double max_norm, double scale, bool adamw, bool zero_grad, int64_t seed) {
-  TORCH_CHECK(params.size() == grads.size() && params.size() == blocks.size() && params.size() == places.size(),
+// params (all of the optimizer's), their gradients (none: left out of the step) and first blocks of moments; lr, step, norm,
+// nonfinite: one float32 each, steps: one for each parameter, ctl: 8 and 4 for each (factors of the step); parts: float64,
+// ticket: int32 (zero)
+void adam_tensors(std::vector<at::Tensor> params, std::vector<OptT> grads, std::vector<int64_t> blocks, std::vector<at::Tensor> state,
+                  at::Tensor lr, at::Tensor step, at::Tensor steps, at::Tensor ctl, at::Tensor norm, at::Tensor nonfinite,
+                  at::Tensor parts, at::Tensor ticket, double beta1, double beta2, double eps, double wd, double max_norm,
+                  double scale, bool adamw, bool zero_grad, bool skip, int64_t seed) {
+  TORCH_CHECK(params.size() == grads.size() && params.size() == blocks.size() && (int64_t)params.size() == steps.numel(),
               "adam_tensors: lists of one length");
   TORCH_CHECK(!state.empty(), "adam_tensors: no state");
   const auto device = state[0].device();
   int64_t end = 0, elements = 0;
-  for (const auto& p : params) elements += p.numel();
+  for (size_t i = 0; i < params.size(); ++i)
+    if (has(grads[i])) elements += params[i].numel();
   const int group = mta_adam_group((long)elements);
   std::vector<AdamTable> tables;
   for (size_t i = 0; i < params.size(); ++i) {
-    const at::Tensor &p = params[i], &g = grads[i];
-    TORCH_CHECK(p.device() == device && g.device() == device, "adam_tensors: tensor ", i, " is not on ", device);
-    TORCH_CHECK(p.is_contiguous() && g.is_contiguous() && p.sizes() == g.sizes(), "adam_tensors: tensor ", i,
-                " and its gradient must be contiguous and of one shape");
-    const int pt = adam_type(p), gt = adam_type(g);
-    TORCH_CHECK(pt == gt || pt == ADAM_F32, "adam_tensors: tensor ", i, "'s gradient must be of its own type");
-    const long n = p.numel(), groups = (n + group - 1) / group;
-    if (n == 0) continue;
+    const at::Tensor& p = params[i];
+    const bool takes = has(grads[i]) && p.numel() > 0;
+    const long n = takes ? p.numel() : 0, groups = (n + group - 1) / group;
+    if (has(grads[i])) {
+      const at::Tensor& g = *grads[i];
+      TORCH_CHECK(p.device() == device && g.device() == device, "adam_tensors: tensor ", i, " is not on ", device);
+      TORCH_CHECK(p.is_contiguous() && g.is_contiguous() && p.sizes() == g.sizes(), "adam_tensors: tensor ", i,
+                  " and its gradient must be contiguous and of one shape");
+      const int pt = adam_type(p), gt = adam_type(g);
+      TORCH_CHECK(pt == gt || pt == ADAM_F32, "adam_tensors: tensor ", i, "'s gradient must be of its own type");
+    }
     TORCH_CHECK(blocks[i] >= 0 && blocks[i] < (int64_t(1) << 32), "adam_tensors: block of tensor ", i);
+    TORCH_CHECK(groups <= 0x7fffffffL, "adam_tensors: tensor ", i, " is too large");
     end = std::max<int64_t>(end, blocks[i] + (n + ADAM_BLOCK - 1) / ADAM_BLOCK);
     if (tables.empty() || tables.back().count == ADAM_TABLE || (long)tables.back().groups + groups > 0x7fffffffL) {
       tables.emplace_back();
       tables.back().count = 0;
+      tables.back().place = (int)i;
       tables.back().group = group;
       tables.back().groups = 0;
     }
     AdamTable& t = tables.back();
-    TORCH_CHECK(groups <= 0x7fffffffL && n < 1L << ADAM_SIZE_BITS, "adam_tensors: tensor ", i, " is too large");
-    TORCH_CHECK(places[i] >= 0 && places[i] < steps.numel() && places[i] < 1L << (64 - ADAM_SIZE_BITS),
-                "adam_tensors: place of tensor ", i);
-    t.p[t.count] = p.data_ptr();
-    t.g[t.count] = g.data_ptr();
-    t.size[t.count] = (uint64_t)n | (uint64_t)places[i] << ADAM_SIZE_BITS;
+    t.p[t.count] = takes ? p.data_ptr() : nullptr;
+    t.g[t.count] = takes ? grads[i]->data_ptr() : nullptr;
+    t.n[t.count] = n;
     t.block[t.count] = (unsigned)blocks[i];
     t.first[t.count] = t.groups;
-    t.type[t.count] = (unsigned char)(pt | gt << 2);
+    t.type[t.count] = takes ? (unsigned char)(adam_type(p) | adam_type(*grads[i]) << 2) : 0;
     t.groups += (unsigned)groups;
     ++t.count;
   }
+  tables.erase(std::remove_if(tables.begin(), tables.end(), [](const AdamTable& t) { return t.groups == 0; }), tables.end());
   if (zero_grad) {  // one workgroup would clear what another still reads
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
     for (const auto& g : grads)
-      if (g.numel()) spans.emplace_back(reinterpret_cast<uintptr_t>(g.data_ptr()), reinterpret_cast<uintptr_t>(g.data_ptr()) + g.nbytes());
+      if (has(g) && g->numel())
+        spans.emplace_back(reinterpret_cast<uintptr_t>(g->data_ptr()), reinterpret_cast<uintptr_t>(g->data_ptr()) + g->nbytes());
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
       TORCH_CHECK(spans[i].first >= spans[i - 1].second, "adam_tensors: gradients that are to be zeroed share memory");
@@ -1417,7 +1421,7 @@ void adam_tensors(std::vector<at::Tensor> params, std::vector<at::Tensor> grads,
   s.beta1 = (float)beta1, s.beta2 = (float)beta2, s.one_beta1 = (float)(1.0 - beta1), s.one_beta2 = (float)(1.0 - beta2);
   s.dbeta1 = beta1, s.dbeta2 = beta2, s.dwd = wd;
   s.eps = (float)eps, s.wd = (float)wd, s.max_norm = max_norm, s.scale = scale;
-  s.decoupled = adamw ? 1 : 0, s.zero_grad = zero_grad ? 1 : 0;
+  s.decoupled = adamw ? 1 : 0, s.zero_grad = zero_grad ? 1 : 0, s.skip = skip ? 1 : 0;
   c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
   mta_adam_tensors(tables.data(), (int)tables.size(), &s, state.size() == 2 ? 1 : 0, cur_stream());
 }

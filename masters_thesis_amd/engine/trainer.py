@@ -267,7 +267,7 @@ class Trainer:
         kw = dict(lr=g["lr"], betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], adamw=adamw)
         # model.optimizer=adam_8bit / adamw_8bit: moments in 8 bits, over the tensors instead of the flat buffer
         narrow = str(getattr(model, "optimizer_kind", "")).endswith("_8bit")
-        self.optimizer = TensorAdam(self.flat.params, state_bits=8, **kw) if narrow else FusedAdam(self.flat, **kw)
+        self.optimizer = TensorAdam(self.flat.params, state_bits=8, skip_nonfinite=True, **kw) if narrow else FusedAdam(self.flat, **kw)
         self.optimizer_name = "AdamW" if adamw else "Adam"
         self.scheduler_cfg = {}
         self.scheduler = None

@@ -352,7 +352,12 @@ class TensorAdam:
     ``state_bits=8``: 256 elements of a tensor share a power of two; an element keeps 4 bits of exponent and 3 (first
     moment, with sign) or 4 (second) of mantissa, rounded up or down by chance so that the mean is right.  The random
     bits are a hash of ``seed``, the step and the element's place: the same run gives the same bits.  2 bytes a
-    parameter instead of 8.  A NaN or infinite gradient makes the moments of its block NaN.
+    parameter instead of 8.
+
+    A NaN or infinite gradient makes its parameter NaN, and in 8 bits the moments of its block; with ``max_norm`` the
+    norm and so every parameter, as ``torch.nn.utils.clip_grad_norm_`` would.  ``skip_nonfinite``: a step whose gradient
+    norm is not finite changes no parameter, moment or count (gradients are zeroed if asked for) and is counted in
+    ``nonfinite``; the norm is then taken without ``max_norm`` too.
 
     ``step(grads=...)`` takes the gradients in the parameters' order; without it, ``p.grad``.  A parameter whose
     gradient is None is left out of the step: each tensor has its own count of steps (``steps``), as in torch.optim.
@@ -360,7 +365,8 @@ class TensorAdam:
     """
 
     def __init__(self, params: Iterable[Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 0.0, adamw: bool = True, state_bits: int = 32, seed: int = 0):
+                 weight_decay: float = 0.0, adamw: bool = True, state_bits: int = 32, seed: int = 0,
+                 skip_nonfinite: bool = False):
         self.params: List[Tensor] = list(params)
         if not self.params:
             raise ValueError("TensorAdam: no parameters")
@@ -380,6 +386,7 @@ class TensorAdam:
                 raise ValueError(f"TensorAdam: parameters {i} and {j} share memory")
         self.betas, self.eps, self.weight_decay = (b1, b2), float(eps), float(weight_decay)
         self.adamw, self.state_bits, self.seed = bool(adamw), int(state_bits), int(seed) & ((1 << 63) - 1)
+        self.skip_nonfinite = bool(skip_nonfinite)
         self._lr = float(lr)
         #: where each tensor's moments start in the buffers of ``moments()`` (whole blocks of 256)
         self.offsets: List[int] = []
@@ -398,7 +405,8 @@ class TensorAdam:
         #: steps taken, and by each tensor
         self.step_t = torch.zeros(1, **f32)
         self.steps = torch.zeros(len(self.params), **f32)
-        #: norm of the last step's scaled gradient, and the count of steps where it was not finite: with ``max_norm`` only
+        #: norm of the last step's scaled gradient, and the count of steps where it was not finite: with ``max_norm`` or
+        #: ``skip_nonfinite`` only
         self.grad_norm = torch.zeros(1, **f32)
         self.nonfinite = torch.zeros(1, **f32)
         self.grads_zeroed = False
@@ -440,33 +448,34 @@ class TensorAdam:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"TensorAdam: {len(grads)} gradients for {len(self.params)} parameters")
-        params, blocks, places = self.params, self._blocks if self.hip else self.offsets, list(range(len(grads)))
-        if any(g is None for g in grads):
-            places = [i for i, g in enumerate(grads) if g is not None]
-            params, blocks, grads = [params[i] for i in places], [blocks[i] for i in places], [grads[i] for i in places]
-        if not grads:
+        if all(g is None for g in grads):
             return
         if not self.hip:
-            self._step_torch(params, blocks, places, grads, max_norm, grad_scale)
+            self._step_torch(grads, max_norm, grad_scale)
             if zero_grad:
                 for g in grads:
-                    g.zero_()
+                    if g is not None:
+                        g.zero_()
         else:
             if not zero_grad:
-                grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-            lib().adam_tensors(params, grads, blocks, places, self._state, self.lr_t, self.step_t, self.steps, self._ctl,
+                grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+            lib().adam_tensors(self.params, grads, self._blocks, self._state, self.lr_t, self.step_t, self.steps, self._ctl,
                                self.grad_norm, self.nonfinite, self._parts, self._ticket, *self.betas, self.eps, self.weight_decay,
-                               float(max_norm or 0.0), float(grad_scale), self.adamw, bool(zero_grad), self.seed)
+                               float(max_norm or 0.0), float(grad_scale), self.adamw, bool(zero_grad), self.skip_nonfinite,
+                               self.seed)
         self.grads_zeroed = bool(zero_grad)
 
-    def _step_torch(self, params, offsets, places, grads, max_norm, grad_scale) -> None:
+    def _step_torch(self, grads, max_norm, grad_scale) -> None:
         b1, b2 = self.betas
         scale = float(grad_scale)
-        if max_norm and max_norm > 0:
-            norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt() * scale
+        if (max_norm and max_norm > 0) or self.skip_nonfinite:
+            norm = torch.stack([g.double().square().sum() for g in grads if g is not None]).sum().sqrt() * scale
             self.grad_norm.copy_(norm.float().reshape(1))
-            if not torch.isfinite(norm):
+            if not torch.isfinite(self.grad_norm):
                 self.nonfinite += 1
+                if self.skip_nonfinite:
+                    return
+        if max_norm and max_norm > 0:
             scale = scale * torch.clamp(max_norm / (norm + 1e-6), max=1.0)
         self.step_t += 1
         m, v = self.moments()
@@ -475,7 +484,9 @@ class TensorAdam:
             kind, m, v = torch.float64, m.double(), v.double()
         chances = torch.zeros(2, self.padded if self.state_bits == 8 else 0, dtype=torch.long, device=m.device)
         took = torch.zeros(self.padded // _BLOCK, dtype=torch.bool, device=m.device)
-        for p, g, o, place in zip(params, grads, offsets, places):
+        for place, (p, g, o) in enumerate(zip(self.params, grads, self.offsets)):
+            if g is None:
+                continue
             if p.shape != g.shape:
                 raise ValueError(f"TensorAdam: parameter {tuple(p.shape)} with gradient {tuple(g.shape)}")
             n = p.numel()

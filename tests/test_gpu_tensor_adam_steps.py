@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_tensor_adam_steps_cpu import SHAPES, run, tensors
+from test_tensor_adam_steps_cpu import SHAPES, check_skipped, run, tensors
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -74,3 +74,30 @@ def test_a_loaded_state_replaces_all_moments(bits):
     assert torch.equal(m[o:o + n].cpu(), full["state"][1]["exp_avg"].view(-1)) and m[o:o + n].any()
     m[o:o + n] = v[o:o + n] = 0
     assert not m.any() and not v.any() and a.steps.tolist() == [0.0, float(full["state"][1]["step"]), 0.0]
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_steps_that_are_not_finite_are_skipped(bits, max_norm):
+    check_skipped(bits, max_norm, DEV)
+
+
+def test_a_captured_step_skips_too():
+    from masters_thesis_amd.ops.optim import TensorAdam
+
+    ps, gs = [p.to(DEV) for p in tensors(SHAPES)], [g.to(DEV) for g in tensors(SHAPES, seed=1)]
+    opt = TensorAdam(ps, lr=1e-2, state_bits=8, skip_nonfinite=True)
+    opt.step(1.0, grads=gs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(1.0, zero_grad=True, grads=gs)
+    for t in range(4):
+        for g, x in zip(gs, tensors(SHAPES, seed=t)):
+            g.copy_(x)
+        if t % 2:
+            gs[1][3, 2] = float("nan")
+        was = [x.clone() for x in ps + opt._state]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(was, ps + opt._state)) == bool(t % 2) and not any(g.any() for g in gs)
+    assert opt.steps.tolist() == [3.0] * 3 and float(opt.nonfinite) == 2

@@ -81,3 +81,60 @@ def test_a_loaded_state_replaces_all_moments(bits):
         gs = tensors(SHAPES, seed=70)
         b.step(grads=gs), fresh.step(grads=gs)
         assert all(torch.equal(x, y) for i, (x, y) in enumerate(zip(b.params, fresh.params)) if i not in keep)
+
+
+def check_skipped(bits, max_norm, device):
+    """A step with a gradient that is not finite changes nothing but the count of such steps (and zeroes the gradients)."""
+    shapes = [(300,), (70, 90), (0,), (1,)]
+    make = lambda seed: [x.to(device) for x in tensors(shapes, seed)]  # noqa: E731
+    a, b = (TensorAdam(make(0), lr=1e-2, state_bits=bits, skip_nonfinite=s) for s in (True, False))
+    for o in (a, b):
+        o.step(max_norm, grads=make(1))
+    state = lambda o: [x.clone() for x in (*o.params, *o._state, o.steps, o.step_t)]  # noqa: E731
+    was, seen = state(a), 0
+    assert all(torch.equal(x, y) for x, y in zip(was, state(b)))
+    for zero in (False, True):
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            for where in (0, 1, 3):
+                gs = make(2)
+                gs[where].view(-1)[-1] = bad
+                a.step(max_norm, zero_grad=zero, grads=gs)
+                seen += 1
+                assert all(torch.equal(x, y) for x, y in zip(was, state(a))) and float(a.nonfinite) == seen
+                assert not torch.isfinite(a.grad_norm).any()
+                assert all(not g.any() for g in gs) if zero else gs[1].any()
+    for o in (a, b):
+        o.step(max_norm, grads=make(3))
+    assert all(torch.equal(x, y) for x, y in zip(state(a), state(b))) and torch.isfinite(a.grad_norm).all()
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_steps_that_are_not_finite_are_skipped(bits, max_norm):
+    check_skipped(bits, max_norm, "cpu")
+
+
+def test_the_trainer_keeps_its_weights_through_a_bad_gradient():
+    """model.optimizer=adam_8bit: one NaN in a gradient loses neither weights nor moments, and is counted."""
+    from masters_thesis_amd.engine import Trainer
+    from masters_thesis_amd.models import get_model_class
+
+    for clip in (None, 5.0):
+        torch.manual_seed(0)
+        model = get_model_class("FinancialLstmMse", "lstm")(input_size=3, hidden_size=32, num_layers=1, dropout=0.0, optimizer="adam_8bit")
+        tr = Trainer(gradient_clip_val=clip, enable_progress_bar=False, enable_model_summary=False, accelerator="cpu")
+        tr._setup_env()
+        tr._setup_model(model)
+        tr._configure_optimizers(model)
+        assert isinstance(tr.optimizer, TensorAdam)
+        tr.flat.grad.normal_()
+        tr._optimizer_step()
+        was = [x.clone() for x in (tr.flat.data, *tr.optimizer._state)]
+        tr.flat.grad.normal_()
+        tr.flat.params[0].grad.view(-1)[3] = float("nan")
+        tr._optimizer_step()
+        assert all(torch.equal(x, y) for x, y in zip(was, (tr.flat.data, *tr.optimizer._state)))
+        assert float(tr.optimizer.nonfinite) == 1 and not any(p.grad.any() for p in tr.flat.params)
+        tr.flat.grad.normal_()
+        tr._optimizer_step()
+        assert torch.isfinite(tr.flat.data).all() and not torch.equal(tr.flat.data, was[0])
