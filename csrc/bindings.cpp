@@ -1424,6 +1424,11 @@ void adam_tensors(std::vector<at::Tensor> params, std::vector<OptT> grads, std::
   s.decoupled = adamw ? 1 : 0, s.zero_grad = zero_grad ? 1 : 0, s.skip = skip ? 1 : 0;
   c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
   mta_adam_tensors(tables.data(), (int)tables.size(), &s, state.size() == 2 ? 1 : 0, cur_stream());
+  for (size_t i = 0; i < params.size(); ++i)
+    if (has(grads[i])) {
+      bump_version(params[i]);
+      if (zero_grad) bump_version(*grads[i]);
+    }
 }
 
 // 8-bit moments as values (read: float32 or bfloat16, which holds every one of them) or from float32 values (write)

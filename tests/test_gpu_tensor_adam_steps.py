@@ -101,3 +101,23 @@ def test_a_captured_step_skips_too():
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(was, ps + opt._state)) == bool(t % 2) and not any(g.any() for g in gs)
     assert opt.steps.tolist() == [3.0] * 3 and float(opt.nonfinite) == 2
+
+
+def test_a_backward_that_saved_what_a_step_changed_sees_it():
+    """Parameters, and gradients that are zeroed; not those that are left as they were."""
+    from masters_thesis_amd.ops.optim import TensorAdam
+
+    ps = [torch.nn.Parameter(p.to(DEV)) for p in tensors(SHAPES)]
+    gs = [g.to(DEV) for g in tensors(SHAPES, seed=1)]
+    opt = TensorAdam(ps, lr=1e-2)
+    x = torch.ones(2, device=DEV, requires_grad=True)
+    late = [(x[0] * p).square().sum() for p in ps] + [(x[1] * g).sum() for g in gs]
+    opt.step(grads=[None, *gs[1:]])
+    late[0].backward(), late[4].backward()
+    for y in late[1:3]:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    opt.step(grads=[None, *gs[1:]], zero_grad=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        late[5].backward()
+    late[3].backward()
