@@ -3,6 +3,7 @@
 #include <stdint.h>
 
 constexpr int ADAM_BLOCK = 256;   // elements of a tensor that share one power of two (8-bit moments)
+constexpr long ADAM_GROUPS = 0xffffff;  // workgroups of one launch: of 256 threads, and a launch holds 2^32 - 1
 constexpr int ADAM_TABLE = 112;   // tensors of one launch: the table travels by value, as kernel arguments (< 4 KB)
 
 // element types of a tensor and its gradient: p | g << 2

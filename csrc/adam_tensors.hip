@@ -25,6 +25,8 @@
 // computed in 64 bits up to their rounding (an element in some 10^6 falls on another code where they are off by an ulp of
 // fp32, and a code is 3 to 6 % of the value), all else in fp32; nothing is contracted, so that the formulas give the same
 // bits wherever they are evaluated.
+#include <initializer_list>
+
 #include "adam_tensors.h"
 #include "common.h"
 
@@ -464,25 +466,35 @@ inline int grid_blocks(long blocks) {
 extern "C" int mta_adam_group(long elements) { return elements < (4L << 20) ? 4 * ADAM_BLOCK : 16 * ADAM_BLOCK; }
 extern "C" int mta_adam_norm_parts() { return NORM_GROUPS; }
 
-// tables: `count` of them.  The norm over all of them first (with clipping or skipping), then the update of each.
-extern "C" void mta_adam_tensors(const AdamTable* tables, int count, const AdamState* s, int wide, hipStream_t st) {
+// tables: `count` of them.  The norm over all of them first (with clipping or skipping), then the update of each.  0, or: 2 a
+// table has more workgroups than a launch, 4 a launch failed
+extern "C" int mta_adam_tensors(const AdamTable* tables, int count, const AdamState* s, int wide, hipStream_t st) {
+  for (int k = 0; k < count; ++k)
+    if (tables[k].groups < 1 || tables[k].groups > ADAM_GROUPS) return 2;
+  auto start = [&](const void* f, unsigned grid, int threads, std::initializer_list<const void*> args) {
+    void* p[8];
+    int n = 0;
+    for (const void* a : args) p[n++] = const_cast<void*>(a);
+    return hipLaunchKernel(f, dim3(grid), dim3(threads), p, 0, st) == hipSuccess;
+  };
   if (s->max_norm > 0.0 || s->skip) {
     int part0 = 0;
     for (int k = 0; k < count; ++k) {
       const long want = ((long)tables[k].groups * tables[k].group + NORM_ELEMENTS - 1) / NORM_ELEMENTS;
-      const int parts = (int)(want < NORM_GROUPS ? want : NORM_GROUPS);
-      adam_norm_kernel<<<parts, NORM_TPB, 0, st>>>(tables[k], *s, part0, part0 + parts, k + 1 == count);
-      part0 += parts;
+      const int parts = (int)(want < NORM_GROUPS ? want : NORM_GROUPS), all = part0 + parts, last = k + 1 == count;
+      if (!start((const void*)adam_norm_kernel, parts, NORM_TPB, {&tables[k], s, &part0, &all, &last})) return 4;
+      part0 = all;
     }
-  } else {
-    adam_factors_kernel<<<1, NORM_TPB, 0, st>>>(*s);
+  } else if (!start((const void*)adam_factors_kernel, 1, NORM_TPB, {s})) {
+    return 4;
   }
   for (int k = 0; k < count; ++k) {
     const bool few = tables[k].group == 4 * ADAM_BLOCK;
     auto kernel = wide ? (few ? adam_update_kernel<true, 1> : adam_update_kernel<true, 4>)
                        : (few ? adam_update_kernel<false, 1> : adam_update_kernel<false, 4>);
-    kernel<<<tables[k].groups, TPB, 0, st>>>(tables[k], *s);
+    if (!start((const void*)kernel, tables[k].groups, TPB, {&tables[k], s})) return 4;
   }
+  return 0;
 }
 
 extern "C" void mta_adam_read(const AdamState* s, void* m, void* v, int bf16, long blocks, hipStream_t st) {

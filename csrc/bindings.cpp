@@ -168,7 +168,7 @@ int mta_rope(int dtype, void* x, long tokens, int seq, long ld, int heads, int D
              hipStream_t st);
 int mta_adam_group(long elements);
 int mta_adam_norm_parts();
-void mta_adam_tensors(const AdamTable* tables, int count, const AdamState* s, int wide, hipStream_t st);
+int mta_adam_tensors(const AdamTable* tables, int count, const AdamState* s, int wide, hipStream_t st);
 void mta_adam_read(const AdamState* s, void* m, void* v, int bf16, long blocks, hipStream_t st);
 void mta_adam_write(const AdamState* s, const float* m, const float* v, long blocks, hipStream_t st);
 }
@@ -1368,9 +1368,9 @@ void adam_tensors(std::vector<at::Tensor> params, std::vector<OptT> grads, std::
       TORCH_CHECK(pt == gt || pt == ADAM_F32, "adam_tensors: tensor ", i, "'s gradient must be of its own type");
     }
     TORCH_CHECK(blocks[i] >= 0 && blocks[i] < (int64_t(1) << 32), "adam_tensors: block of tensor ", i);
-    TORCH_CHECK(groups <= 0x7fffffffL, "adam_tensors: tensor ", i, " is too large");
+    TORCH_CHECK(groups <= ADAM_GROUPS, "adam_tensors: tensor ", i, " is too large for one launch");
     end = std::max<int64_t>(end, blocks[i] + (n + ADAM_BLOCK - 1) / ADAM_BLOCK);
-    if (tables.empty() || tables.back().count == ADAM_TABLE || (long)tables.back().groups + groups > 0x7fffffffL) {
+    if (tables.empty() || tables.back().count == ADAM_TABLE || (long)tables.back().groups + groups > ADAM_GROUPS) {
       tables.emplace_back();
       tables.back().count = 0;
       tables.back().place = (int)i;
@@ -1423,7 +1423,8 @@ void adam_tensors(std::vector<at::Tensor> params, std::vector<OptT> grads, std::
   s.eps = (float)eps, s.wd = (float)wd, s.max_norm = max_norm, s.scale = scale;
   s.decoupled = adamw ? 1 : 0, s.zero_grad = zero_grad ? 1 : 0, s.skip = skip ? 1 : 0;
   c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
-  mta_adam_tensors(tables.data(), (int)tables.size(), &s, state.size() == 2 ? 1 : 0, cur_stream());
+  const int rc = mta_adam_tensors(tables.data(), (int)tables.size(), &s, state.size() == 2 ? 1 : 0, cur_stream());
+  TORCH_CHECK(rc == 0, "adam_tensors: not launched (rc=", rc, ")");
   for (size_t i = 0; i < params.size(); ++i)
     if (has(grads[i])) {
       bump_version(params[i]);

@@ -414,7 +414,8 @@ class TensorAdam:
         if self.hip:
             C = lib()
             self._blocks = [o // _BLOCK for o in self.offsets]
-            launches = -(-len(self.params) // C.ADAM_TABLE) + sum(p.numel() >> 42 for p in self.params)
+            # tables of a step: by their tensors, and where their workgroups fill a launch (16 Mi of at least 1024 elements)
+            launches = -(-len(self.params) // C.ADAM_TABLE) + sum(1 + (p.numel() >> 33) for p in self.params if p.numel() >> 30)
             self._parts = torch.zeros(launches * C.adam_norm_parts(), device=dev, dtype=torch.float64)
             self._ticket = torch.zeros(1, device=dev, dtype=torch.int32)
             self._ctl = torch.zeros(8 + 4 * len(self.params), **f32)

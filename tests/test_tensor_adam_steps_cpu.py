@@ -1,4 +1,6 @@
 """ops.optim.TensorAdam: tensors that start late or are left out, and states of part of the tensors, as torch.optim has them."""
+import ctypes
+
 import pytest
 import torch
 
@@ -138,3 +140,25 @@ def test_the_trainer_keeps_its_weights_through_a_bad_gradient():
         tr.flat.grad.normal_()
         tr._optimizer_step()
         assert torch.isfinite(tr.flat.data).all() and not torch.equal(tr.flat.data, was[0])
+
+
+class Table(ctypes.Structure):  # csrc/adam_tensors.h AdamTable
+    _fields_ = [("p", ctypes.c_void_p * 112), ("g", ctypes.c_void_p * 112), ("n", ctypes.c_long * 112), ("block", ctypes.c_uint * 112),
+                ("first", ctypes.c_uint * 112), ("type", ctypes.c_ubyte * 112), ("count", ctypes.c_int), ("place", ctypes.c_int),
+                ("group", ctypes.c_int), ("groups", ctypes.c_uint)]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="host checks: a launch would run")
+@pytest.mark.parametrize("groups", [0, 2 ** 24, 2 ** 31])
+def test_more_workgroups_than_a_launch_holds(groups):
+    """Refused before anything is started; and a launch that fails (here: no device) is told."""
+    from masters_thesis_amd.ops import build
+    from masters_thesis_amd.ops._lib import lib
+
+    lib()
+    so = ctypes.CDLL(str(build.ext_path()))
+    so.mta_adam_tensors.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    t, state = Table(count=1, group=4096, groups=groups), ctypes.create_string_buffer(512)
+    assert so.mta_adam_tensors(ctypes.byref(t), 1, state, 1, None) == 2
+    t.groups = 5
+    assert so.mta_adam_tensors(ctypes.byref(t), 1, state, 1, None) == 4
