@@ -43,6 +43,20 @@ def env_world_size() -> int:
     return int(os.environ.get("WORLD_SIZE", "1"))
 
 
+def ranks_share_gpus(local_world: int, devices: int) -> bool:
+    """Whether ranks of this machine share GPUs (a rehearsal on fewer GPUs than ranks); if so, defaults for it.
+
+    The hardware runs the processes on a GPU side by side or in turns, so a workgroup that polls for another of its own launch
+    may keep the other from running: the pipelined LSTM's hand-offs then give up after their bound, or take minutes to get
+    through a step.  Ranks that share a GPU take the per-layer LSTM kernels, which wait for nothing inside a launch, and the
+    optimizer's one grid-wide wait polls longer (as for trials that share a GPU, ``config/app.py``)."""
+    if not 0 < devices < local_world:
+        return False
+    os.environ.setdefault("MTA_LSTM_PIPELINE", "0")
+    os.environ.setdefault("MTA_ADAM_SPIN_LIMIT", str(1 << 26))
+    return True
+
+
 def init_distributed(backend: Optional[str] = None, timeout_s: float = 600.0, device: Optional[str] = None) -> DistEnv:
     """Initialise (once) from torchrun-style env vars; returns the rank/device description."""
     global _ENV
@@ -63,7 +77,7 @@ def init_distributed(backend: Optional[str] = None, timeout_s: float = 600.0, de
     if world > 1:
         # RCCL needs one GPU per rank: ranks sharing a GPU (a rehearsal on fewer GPUs than ranks) take gloo for the
         # host collectives; their gradient sync is still the xGMI/IPC kernel (parallel/ddp.py)
-        shared = use_gpu and int(os.environ.get("LOCAL_WORLD_SIZE", world)) > torch.cuda.device_count()
+        shared = use_gpu and ranks_share_gpus(int(os.environ.get("LOCAL_WORLD_SIZE", world)), torch.cuda.device_count())
         be = backend or os.environ.get("MTA_DIST_BACKEND") or ("nccl" if use_gpu and not shared else "gloo")
         os.environ.setdefault("TORCH_NCCL_ASYNC_ERROR_HANDLING", "1")
         if not dist.is_initialized():

@@ -155,3 +155,19 @@ def test_xgmi_range_channel_invariant():
     assert ddp.channel_of(0, 1024) == 0 and ddp.channel_of(1024, 4096) == 1
     with pytest.raises(RuntimeError, match="channel invariant"):
         ddp.channel_of(0, 4096)
+
+
+@pytest.mark.parametrize("ranks,devices,shared", [(2, 1, True), (8, 4, True), (1, 1, False), (8, 8, False), (2, 0, False)])
+def test_ranks_that_share_a_gpu_take_kernels_without_waits(ranks, devices, shared, monkeypatch):
+    """Polling workgroups of two processes on one GPU hold each other up; what the caller set himself stays."""
+    from masters_thesis_amd.parallel import dist as pdist
+
+    for given in (None, "1"):
+        for k in ("MTA_LSTM_PIPELINE", "MTA_ADAM_SPIN_LIMIT"):
+            monkeypatch.setenv(k, "x")  # so that it is restored
+            monkeypatch.delenv(k)
+        if given:
+            monkeypatch.setenv("MTA_LSTM_PIPELINE", given)
+        assert pdist.ranks_share_gpus(ranks, devices) == shared
+        assert os.environ.get("MTA_LSTM_PIPELINE") == (given or ("0" if shared else None))
+        assert ("MTA_ADAM_SPIN_LIMIT" in os.environ) == shared
