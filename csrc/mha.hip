@@ -250,8 +250,8 @@ __device__ __forceinline__ float half_sum(float x) {
   return lo + hi;
 }
 
-// values 8 s .. 8 s + 7 of an accumulator as the next product's operand.  Rounded to 16 bits here (half a step, 2^-9 /
-// 2^-12 of each value); sums of the same values are taken from the unrounded ones.
+// values 8 s .. 8 s + 7 of an accumulator as the next product's operand.  Rounded to 16 bits here (half a step, 2^-8 /
+// 2^-11 of each value); sums of the same values are taken from the unrounded ones.
 template <typename T>
 __device__ __forceinline__ typename El<T>::frag as_frag(const f32x16& a, int s) {
   typename El<T>::frag f;

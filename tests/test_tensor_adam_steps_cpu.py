@@ -162,3 +162,28 @@ def test_more_workgroups_than_a_launch_holds(groups):
     assert so.mta_adam_tensors(ctypes.byref(t), 1, state, 1, None) == 2
     t.groups = 5
     assert so.mta_adam_tensors(ctypes.byref(t), 1, state, 1, None) == 4
+
+
+def test_moments_in_8_bits_against_32_over_many_steps():
+    """The same gradients for 600 steps: rounding by chance keeps the mean, and what noise it leaves has a bound.
+
+    A step moves v by (1 - b2) |g^2 - v|, on average 0.97 (1 - b2) v for normal gradients; rounded up or down on a grid of
+    steps s <= v / 16, the chance of the nearer end is that part of s, so the variance added is at most s 0.97 (1 - b2) v, and
+    what stays of all steps' is 1 / (1 - b2^2) of it: 0.97 / 32 v^2, a deviation of 0.175 v.  m likewise with steps of |m| / 8,
+    at most one step's s^2 / 4 a time: (m_max / 8)^2 / 4 / (1 - b1^2) of the block's largest m."""
+    n, b1, b2 = 8192, 0.9, 0.99
+    ps = [torch.zeros(n), torch.zeros(n)]
+    opts = [TensorAdam([p], lr=1e-3, betas=(b1, b2), state_bits=bits, seed=11) for p, bits in zip(ps, (8, 32))]
+    size = torch.linspace(0.5, 2.0, n)
+    g = torch.Generator().manual_seed(0)
+    for _ in range(600):
+        x = torch.randn(n, generator=g) * size
+        for o in opts:
+            o.step(grads=[x])
+    (m8, v8), (m, v) = opts[0].moments(), opts[1].moments()
+    off = (v8 / v - 1).double()
+    assert float(off.std()) <= 0.175 * 1.03 and abs(float(off.mean())) <= 5 * 0.175 / n ** 0.5
+    top = m.view(-1, 256).abs().amax(1, keepdim=True).expand(-1, 256).reshape(-1)
+    off = ((m8 - m) / top).double()
+    noise = 1 / 8 / 2 / (1 - b1 ** 2) ** 0.5
+    assert float(off.std()) <= noise and abs(float(off.mean())) <= 5 * noise / n ** 0.5
