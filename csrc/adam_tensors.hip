@@ -21,7 +21,7 @@
 // A block with a NaN or an infinity reads as NaN afterwards.
 //
 // Bound by memory: 28 bytes an fp32 parameter (p, m, v read and written, g read), 16 in 8 bits: 403 million weights in
-// 1.35 ms, 4.8 TB/s (a copy: 4.7).  The norm is a pass of its own, 52 us for 64 million bf16 gradients.  Moments in 8 bits are
+// 1.32 ms, 4.9 TB/s (a copy: 4.7 - 4.8).  The norm is a pass of its own, 51 us for 64 million bf16 gradients.  Moments in 8 bits are
 // computed in 64 bits up to their rounding (an element in some 10^6 falls on another code where they are off by an ulp of
 // fp32, and a code is 3 to 6 % of the value), all else in fp32; nothing is contracted, so that the formulas give the same
 // bits wherever they are evaluated.

@@ -529,8 +529,8 @@ __device__ __forceinline__ void wave_order() {
 
 // Few rows: 32 of a problem to a workgroup; every wave takes all of them and every fourth 32-key block of the workgroup's
 // range, through LDS of its own, so that nothing waits for the other waves; their sums are joined at the end.  One query
-// against 16 caches of up to 32768 keys, 32 heads of 128 on 8, bf16: 298 us, 4.5 TB/s, bound by memory, and 7 us for the
-// join of its ranges.
+// against 16 caches of up to 32768 keys, 32 heads of 128 on 8, bf16: 298 us for 1573 MB, 5.3 TB/s, bound by memory,
+// and 7 us for the join of its ranges.
 template <typename T, int DP>
 __global__ __launch_bounds__(THREADS, forward_waves<T>(DP)) void mha_few_kernel(MhaArgs A) {
   typedef Tile<T, DP> TL;
@@ -819,7 +819,7 @@ struct GradRows {
 };
 
 // Many rows: 128 of a problem to a workgroup, 32 to a wave, walking the key tiles (4096 tokens causal, 32 heads of 128 on
-// 8, bf16: 350 us, 0.59 PFLOP/s with one wave a SIMD; 6 x 1500, 8 of 64, fp16: 51 us); dq_splits > 1: a range of
+// 8, bf16: 354 us, 0.58 PFLOP/s with one wave a SIMD; 6 x 1500, 8 of 64, fp16: 50 us); dq_splits > 1: a range of
 // them, summed by a further launch
 template <typename T, int DP, int BN>
 __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dq_kernel(MhaArgs A) {
@@ -1245,7 +1245,7 @@ struct Walk {
 
 // Many keys: 128 of a problem to a workgroup, 32 to a wave, walking the rows in tiles of BR.  With causal order key tile i
 // is seen by fewer rows the later it is: a workgroup takes tiles i and N - 1 - i, whose rows add up to the same number for
-// every i.  (The two calls above: 386 us, 0.71 PFLOP/s, and 72 us.)  kv_splits > 1: a kv_splits-th of each tile's rows,
+// every i.  (The two calls above: 379 us, 0.73 PFLOP/s, and 70 us.)  kv_splits > 1: a kv_splits-th of each tile's rows,
 // summed by a further launch.
 template <typename T, int DP, int BR>
 __global__ __launch_bounds__(THREADS, backward_waves<T>(DP)) void mha_dkv_kernel(MhaArgs A) {
