@@ -20,6 +20,8 @@ def _lib():
     from masters_thesis_amd.ops import build
     from masters_thesis_amd.ops._lib import lib
 
+    if not build.ext_path().exists():
+        build.build()
     lib()
     so = ctypes.CDLL(str(build.ext_path()))
     so.mta_mha_plan.restype = ctypes.c_long

@@ -155,6 +155,8 @@ def test_more_workgroups_than_a_launch_holds(groups):
     from masters_thesis_amd.ops import build
     from masters_thesis_amd.ops._lib import lib
 
+    if not build.ext_path().exists():
+        build.build()
     lib()
     so = ctypes.CDLL(str(build.ext_path()))
     so.mta_adam_tensors.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
