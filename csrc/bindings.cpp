@@ -1063,7 +1063,8 @@ double mha_check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
                       lens->sizes(), " on ", lens->device());
   TORCH_CHECK_NOT_IMPLEMENTED(!mha_dual({&q, &k, &v}), "attention: no forward-mode derivatives on the GPU");
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)D);
-  TORCH_CHECK_VALUE(s > 0 && std::isfinite(s), "attention: scale must be positive, got ", s);
+  // (in float32, times log2(e), it is neither 0 nor infinite: 0 times a hidden score would be a NaN)
+  TORCH_CHECK_VALUE(s >= 0x1p-120 && s <= 0x1p120, "attention: scale must be positive, 2^-120 to 2^120, got ", s);
   return s;
 }
 

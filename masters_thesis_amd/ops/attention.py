@@ -52,8 +52,8 @@ def _check(q: Tensor, k: Tensor, v: Tensor, key_lengths: Optional[Tensor], scale
         if key_lengths.device != q.device:
             raise ValueError(f"attention: key_lengths is on {key_lengths.device}, q on {q.device}")
     scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"attention: scale must be positive, got {scale}")
+    if not 2.0 ** -120 <= scale <= 2.0 ** 120:  # a number that float32 holds
+        raise ValueError(f"attention: scale must be positive, 2^-120 to 2^120, got {scale}")
     return scale
 
 
@@ -203,8 +203,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False, key_leng
     what lies behind them is never read as a number (it may be NaN) and gets zero gradients; lengths outside 0 .. Tk
     are clamped.  (A NaN or infinity within the lengths may reach queries whose causal order hides its key, and one in a
     query or its output gradient the gradients of keys that are hidden from it.)  A query that sees no key returns 0,
-    log-sum-exp -inf, and contributes no gradient, whatever it and its output gradient hold.  ``scale``: positive, default
-    ``1 / sqrt(dim)``.
+    log-sum-exp -inf, and contributes no gradient, whatever it and its output gradient hold.  ``scale``: positive (2^-120 to
+    2^120), default ``1 / sqrt(dim)``.
 
     ``return_lse``: also the log-sum-exp (batch, heads, Tq), float32, not differentiable.
 

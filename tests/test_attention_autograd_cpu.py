@@ -65,3 +65,12 @@ def test_what_blind_rows_hold_reaches_nothing():
     for bad in (math.nan, math.inf):
         q[:, :5:2], do[:, 1:5], do[:, 0] = bad, bad, bad
         assert all(torch.equal(a, b) for a, b in zip(run(), want))
+
+
+def test_scales_that_float32_does_not_hold_are_refused():
+    q, k, v = (x.detach() for x in leaves())
+    for scale in (1e-60, 2.0 ** -121, 2.0 ** 121, 1e39, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            attention(q, k, v, scale=scale)
+    even = attention(q, k, v, scale=2.0 ** -120)  # every key weighs the same
+    assert torch.allclose(even, v.mean(1, keepdim=True).repeat_interleave(2, 2).expand_as(even), atol=1e-6)

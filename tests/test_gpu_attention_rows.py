@@ -135,3 +135,15 @@ def test_float16_kernels_of_few_problems_past_dim_64(b, tq, tk, h, hk, causal, f
     names = [e.key for e in prof.key_averages()]
     assert any("mha_dkv_few_kernel" in n for n in names) == few == any("mha_dq_few_kernel" in n for n in names)
     assert any("mha_dkv_kernel" in n for n in names) != few
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scales(dtype):
+    """The smallest scale (every key weighs the same, hidden ones nothing) and the refusal of those that float32 does not hold."""
+    q, k, v, do = make(2, 70, 90, 4, 2, 40, dtype)
+    n = torch.tensor([90, 41], device=DEV)
+    for scale in (1e-60, 2.0 ** -121, 2.0 ** 121, 1e39, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            _A().attention(q, k, v, scale=scale)
+    for causal in (False, True):
+        check(run(q, k, v, do, causal=causal, key_lengths=n, scale=2.0 ** -120), oracle(q, k, v, do, causal, [90, 41], 2.0 ** -120))
