@@ -372,9 +372,7 @@ class TensorAdam:
             raise ValueError("TensorAdam: no parameters")
         if state_bits not in (8, 32):
             raise ValueError(f"TensorAdam: state_bits must be 8 or 32, got {state_bits}")
-        b1, b2 = (float(b) for b in betas)
-        if not (0 <= b1 < 1 and 0 <= b2 < 1 and lr >= 0 and eps > 0 and weight_decay >= 0):
-            raise ValueError(f"TensorAdam: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+        b1, b2 = self._checked(lr, betas, eps, weight_decay)
         dev = self.params[0].device
         for i, p in enumerate(self.params):
             if p.device != dev or p.dtype not in (torch.float32, torch.bfloat16, torch.float16) or not p.is_contiguous():
@@ -424,6 +422,14 @@ class TensorAdam:
             "maximize": False, "foreach": None, "capturable": True, "differentiable": False, "fused": True,
             "decoupled_weight_decay": self.adamw, "params": list(range(len(self.params))),
         }]
+
+    @staticmethod
+    def _checked(lr, betas, eps, weight_decay) -> tuple:
+        b1, b2 = (float(b) for b in betas)
+        # eps: a normal number of float32, as the reciprocal of what is not is taken for that of 0
+        if not (0 <= b1 < 1 and 0 <= b2 < 1 and lr >= 0 and eps >= 2.0 ** -126 and weight_decay >= 0):
+            raise ValueError(f"TensorAdam: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+        return b1, b2
 
     # ---- lr (device-resident) --------------------------------------------------
     @property
@@ -552,9 +558,9 @@ class TensorAdam:
         """Moments go to the nearest code in 8 bits (a state of this optimizer's own: to the values it had).  Tensors that
         the state has no entry of start anew."""
         g = sd["param_groups"][0]
-        self.betas = tuple(float(b) for b in g.get("betas", self.betas))
-        self.eps = float(g.get("eps", self.eps))
-        self.weight_decay = float(g.get("weight_decay", self.weight_decay))
+        eps, decay = float(g.get("eps", self.eps)), float(g.get("weight_decay", self.weight_decay))
+        self.betas = self._checked(g["lr"], g.get("betas", self.betas), eps, decay)
+        self.eps, self.weight_decay = eps, decay
         self.param_groups[0].update(betas=self.betas, eps=self.eps, weight_decay=self.weight_decay)
         self.set_lr(g["lr"])
         m, v = self.moments()

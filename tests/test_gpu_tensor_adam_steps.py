@@ -121,3 +121,16 @@ def test_a_backward_that_saved_what_a_step_changed_sees_it():
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         late[5].backward()
     late[3].backward()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_the_smallest_eps(bits):
+    """Elements without a gradient stay where they are."""
+    from masters_thesis_amd.ops.optim import TensorAdam
+
+    ps = [p.to(DEV) for p in tensors(SHAPES)]
+    was = [p.clone() for p in ps]
+    opt = TensorAdam(ps, lr=1e-2, eps=2.0 ** -126, state_bits=bits, weight_decay=0.0)
+    for _ in range(2):
+        opt.step(grads=[torch.zeros_like(p) for p in ps])
+    assert all(torch.equal(p, w) for p, w in zip(ps, was))

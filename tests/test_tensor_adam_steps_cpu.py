@@ -189,3 +189,17 @@ def test_moments_in_8_bits_against_32_over_many_steps():
     off = ((m8 - m) / top).double()
     noise = 1 / 8 / 2 / (1 - b1 ** 2) ** 0.5
     assert float(off.std()) <= noise and abs(float(off.mean())) <= 5 * noise / n ** 0.5
+
+
+def test_an_eps_that_is_no_normal_number_is_refused():
+    """Also from a state: an element without a gradient would become 0 / 0."""
+    for eps in (1e-46, 2.0 ** -127, 0.0):
+        with pytest.raises(ValueError, match="eps"):
+            TensorAdam(tensors(SHAPES), eps=eps)
+    opt = TensorAdam(tensors(SHAPES), eps=2.0 ** -126)
+    opt.step(grads=[torch.zeros(s) for s in SHAPES])
+    assert all(torch.isfinite(p).all() for p in opt.params)
+    sd = opt.state_dict()
+    for bad in (dict(eps=0.0), dict(betas=(0.9, 1.0)), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            opt.load_state_dict({**sd, "param_groups": [{**sd["param_groups"][0], **bad}]})
